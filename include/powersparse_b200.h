@@ -217,6 +217,91 @@ int ps_ipc_close(void* base);
  * single-GPU; its only device choice is benchmarks/benchmark.cu:116). */
 int ps_partition_rows(int row_num, const int* row_ptr, int parts, int* cuts);
 
+/* --- Rows chosen by an index that the model makes --------------------------------
+ * No reference counterparts.  Products with a sparse matrix that is new in every
+ * call, so there is nothing to preprocess: the operators take device arrays only and
+ * run on the current device, asynchronously on `stream`.  A matrix argument is rows
+ * of `width` elements of type `dtype`, `stride` elements apart (stride >= width,
+ * width <= 2^24); byte offsets are 64-bit.  Sums, products and softmax statistics
+ * are FP32, rounded once, to nearest even, where they are stored.  No call allocates
+ * device memory, waits for the device or uses atomics whose order matters: equal
+ * inputs give equal bits, and every call can be captured into a graph.  Rows that
+ * begin at multiples of 16 bytes, with a width that is a multiple of 16 bytes, are
+ * moved 16 bytes a thread; others by smaller words. */
+enum { PS_F32 = 0, PS_BF16 = 1, PS_F16 = 2 }; /* element types */
+enum { PS_I32 = 0, PS_I64 = 1 };              /* index types */
+
+/* out[i, :] = scale * table[tokens[i], :] for i < n.  table is [rows x width], out
+ * [n x width], both of `dtype`.  A token outside [0, rows) is an empty place (padding,
+ * or a token that another GPU's part of the table holds): its row is zeros. */
+int ps_embedding(const void* table, int dtype, long long rows, int width, long long table_stride, const void* tokens,
+                 int index_type, long long n, float scale, void* out, long long out_stride, void* stream);
+
+/* Gradient of ps_embedding for the table: grad_table[v, :] = scale * sum of grad[i, :]
+ * over the i with tokens[i] = v, summed in FP32 in an order that the batch alone
+ * fixes.  Tokens outside [0, rows), and the token `padding` where that is >= 0, take
+ * no part.  accumulate = 0 writes every row of grad_table (zeros where no token
+ * is); accumulate != 0 adds to the rows that tokens name and leaves the others.
+ * grad_table's type is grad's or PS_F32.  rows <= 2^31 - 2.  workspace: at least
+ * ps_embedding_grad_workspace(n, rows, width) bytes of device memory at a multiple
+ * of 256 (-1 for arguments out of range), in use until the call has run; it needs
+ * no initialisation and nothing in it outlives the call. */
+long long ps_embedding_grad_workspace(long long n, long long rows, int width);
+int ps_embedding_grad(const void* grad, int grad_dtype, long long grad_stride, const void* tokens, int index_type, long long n,
+                      float scale, long long padding, int accumulate, void* grad_table, int table_dtype, long long table_stride,
+                      long long rows, int width, void* workspace, long long workspace_bytes, void* stream);
+
+/* The router of a mixture layer: for every token, the top_k experts of largest score
+ * in descending order (of equal scores the lower index first) and their weights, the
+ * softmax over all experts (normalize = 0) or over the chosen ones (normalize != 0).
+ * logits: [tokens x experts] of `dtype`; weights and chosen: [tokens x top_k], packed.
+ * A score of -inf switches an expert off: where fewer than top_k are left, the last
+ * choices are -1 with weight 0.  A NaN is never chosen, and it makes the weights of its
+ * row NaN, as +inf does.  experts <= 1024, top_k <= min(experts, 32). */
+int ps_route(const void* logits, int dtype, long long logits_stride, int tokens, int experts, int top_k, int normalize,
+             float* weights, int* chosen, void* stream);
+
+/* Gradient of ps_route for the logits, given its outputs and the gradient of the
+ * weights.  Writes all of grad_logits (the type of logits).  The logits are read where
+ * normalize = 0 only.  grad_weights beside a choice of -1 is not used. */
+int ps_route_grad(const float* grad_weights, const void* logits, int dtype, long long logits_stride, const float* weights,
+                  const int* chosen, int tokens, int experts, int top_k, int normalize, void* grad_logits,
+                  long long grad_logits_stride, void* stream);
+
+/* Rows that `slots` = tokens * top_k places can fill at the most when every expert's
+ * rows begin at a multiple of `align` (-1 for arguments out of range). */
+long long ps_dispatch_rows(long long slots, int experts, int align);
+
+/* Tokens copied into the order of their experts: rows[position[t, j], :] = x[t, :] for
+ * every token t and j < top_k.  chosen: [tokens x top_k] indices, packed; one outside
+ * [0, experts) is dropped (position -1).  Expert e's rows begin at offsets[e], a
+ * multiple of align, and hold its counts[e] tokens in the order of the batch; rows up
+ * to offsets[e + 1] are zeros; offsets[experts] is the end.  Rows from there on are set
+ * to zeros too (zero_tail != 0) or stay as they were.  rows: [row_count x width] with row_count >= ps_dispatch_rows(tokens *
+ * top_k, experts, align).  position: tokens * top_k ints, offsets: experts + 1,
+ * counts: experts.  A token may name an expert twice.  experts <= 1024, top_k <= 32,
+ * align <= 65536. */
+int ps_dispatch(const void* x, int dtype, long long x_stride, const void* chosen, int index_type, int tokens, int top_k,
+                int experts, int align, int width, void* rows, long long rows_stride, long long row_count, int zero_tail,
+                int* position, int* offsets, int* counts, void* stream);
+
+/* The experts' rows brought back: out[t, :] = add[t, :] + sum over j of weights[t, j] *
+ * y[position[t, j], :], summed in the order of j.  weights NULL: ones, which makes it
+ * the gradient of ps_dispatch; add NULL: zeros; add may be out itself.  A position
+ * outside [0, row_count) is skipped, and neither its weight nor a row is read for it. */
+int ps_combine(const void* y, int dtype, long long y_stride, long long row_count, const int* position, const float* weights,
+               const void* add, long long add_stride, int tokens, int top_k, int width, void* out, long long out_stride,
+               void* stream);
+
+/* Gradient of ps_combine for y and the weights: grad_y[position[t, j], :] = weights[t, j]
+ * * grad[t, :], grad_weights[t, j] = <grad[t, :], y[position[t, j], :]> (0 for a skipped
+ * position).  position, offsets and counts are ps_dispatch's: the rows between an
+ * expert's tokens and the next expert are set to zeros, and zero_tail says the same
+ * of the rows from offsets[experts] on as there.  (The gradient for add is grad itself.) */
+int ps_combine_grad(const void* grad, int dtype, long long grad_stride, const void* y, long long y_stride, long long row_count,
+                    const int* position, const int* offsets, const int* counts, int experts, const float* weights, int tokens,
+                    int top_k, int width, void* grad_y, long long grad_y_stride, int zero_tail, float* grad_weights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,13 @@ and the additions after the path (no reference counterpart):
     PowerSparseMatrixGPU.save(path) / .load(path)   layout cache
     partition_rows(row_ptr, parts)             nnz-balanced row panels (multi-GPU)
 
+and the operators on rows chosen by an index that the model makes (``powersparse_b200.rows``,
+on torch CUDA tensors; loaded, with torch, at their first use):
+
+    embedding, embedding_grad                  rows of a table by token, and the table's gradient
+    route, route_grad                          a router's softmax and top-k
+    dispatch, dispatch_grad, combine, combine_grad   tokens to their experts and back
+
 ``powersparse_b200.torch_ops`` registers the operators as ``torch.ops.powersparse.*``
 and ``powersparse_b200.distributed`` shards them by row panels over torch.distributed.
 
@@ -37,6 +44,8 @@ import numpy as np
 __all__ = [
     "PowerSparseMatrixGPU", "SpMM", "SDDMM", "SDDMM_csr", "SpMM_values", "edge_softmax_csr", "partition_rows",
     "load_library", "LIB_PATH",
+    "embedding", "embedding_grad", "route", "route_grad", "DispatchPlan", "dispatch_rows", "dispatch",
+    "dispatch_grad", "combine", "combine_grad",
     "GROUP_SIZE", "PS_OK", "PS_ERR_INVALID_ARGUMENT", "PS_ERR_CUDA",
 ]
 
@@ -48,6 +57,7 @@ PS_OK, PS_ERR_INVALID_ARGUMENT, PS_ERR_CUDA, PS_ERR_INTERNAL = 0, 1, 2, 3
 _i32p = ctypes.POINTER(ctypes.c_int)
 _f32p = ctypes.POINTER(ctypes.c_float)
 _vp = ctypes.c_void_p
+_int, _ll, _flt = ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 _lib = None
 
 # (name, restype, argtypes) of every entry point in include/powersparse_b200.h.
@@ -88,7 +98,29 @@ _SIGNATURES = [
     ("ps_ipc_export", ctypes.c_int, [_vp, ctypes.c_char_p, ctypes.POINTER(ctypes.c_ulonglong)]),
     ("ps_ipc_open", ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     ("ps_ipc_close", ctypes.c_int, [_vp]),
+    ("ps_embedding", _int, [_vp, _int, _ll, _int, _ll, _vp, _int, _ll, _flt, _vp, _ll, _vp]),
+    ("ps_embedding_grad_workspace", _ll, [_ll, _ll, _int]),
+    ("ps_embedding_grad", _int, [_vp, _int, _ll, _vp, _int, _ll, _flt, _ll, _int, _vp, _int, _ll, _ll, _int, _vp, _ll, _vp]),
+    ("ps_route", _int, [_vp, _int, _ll, _int, _int, _int, _int, _vp, _vp, _vp]),
+    ("ps_route_grad", _int, [_vp, _vp, _int, _ll, _vp, _vp, _int, _int, _int, _int, _vp, _ll, _vp]),
+    ("ps_dispatch_rows", _ll, [_ll, _int, _int]),
+    ("ps_dispatch", _int, [_vp, _int, _ll, _vp, _int, _int, _int, _int, _int, _int, _vp, _ll, _ll, _int, _vp, _vp, _vp, _vp]),
+    ("ps_combine", _int, [_vp, _int, _ll, _ll, _vp, _vp, _vp, _ll, _int, _int, _int, _vp, _ll, _vp]),
+    ("ps_combine_grad", _int, [_vp, _int, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _int, _vp, _int, _int, _int, _vp, _ll, _int, _vp,
+                               _vp]),
 ]
+
+# Names of powersparse_b200.rows, looked up at their first use: that module needs torch.
+_ROW_OPERATORS = ("embedding", "embedding_grad", "route", "route_grad", "DispatchPlan", "dispatch_rows", "dispatch",
+                  "dispatch_grad", "combine", "combine_grad")
+
+
+def __getattr__(name: str):
+    if name in _ROW_OPERATORS:
+        from . import rows
+        globals().update({n: getattr(rows, n) for n in _ROW_OPERATORS})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 PS_IPC_HANDLE_BYTES = 64
 

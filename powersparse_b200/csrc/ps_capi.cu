@@ -6,6 +6,7 @@
 #include "ps_common.cuh"
 #include "ps_matrix.h"
 #include "ps_ops.h"
+#include "ps_rows.h"
 
 #include <algorithm>
 #include <cstring>
@@ -66,6 +67,45 @@ void require_device(const psb::Matrix& m) {
   if (dev != m.device)
     throw std::invalid_argument("The matrix lives on CUDA device " + std::to_string(m.device) +
                                 " but device " + std::to_string(dev) + " is current");
+}
+
+// Checks of the row operators' arguments; `what` names the operator in the message.
+void require(bool ok, const char* what, const char* text) {
+  if (!ok) throw std::invalid_argument(std::string(what) + ": " + text);
+}
+
+int size_of(int dtype, const char* what) {
+  require(dtype == PS_F32 || dtype == PS_BF16 || dtype == PS_F16, what, "the element type is PS_F32, PS_BF16 or PS_F16");
+  return dtype == PS_F32 ? 4 : 2;
+}
+
+// Rows of `width` elements of `size` bytes at `ptr`, `stride` apart; `rows` of them.
+void require_rows(const void* ptr, long long stride, long long rows, int width, int size, const char* what) {
+  require(rows >= 0 && width >= 1 && width <= (1 << 24), what, "rows must be >= 0 and the width in [1, 2^24]");
+  require(stride >= width && stride < (1LL << 40), what, "the row stride must be at least the width");
+  require(ptr != nullptr || rows == 0, what, "null buffer");
+  require(reinterpret_cast<uintptr_t>(ptr) % size == 0, what, "a buffer is not aligned to its element type");
+}
+
+template <typename T>
+void require_array(const T* ptr, long long count, const char* what) {
+  require(ptr != nullptr || count == 0, what, "null buffer");
+  require(reinterpret_cast<uintptr_t>(ptr) % sizeof(T) == 0, what, "a buffer is not aligned to its element type");
+}
+
+psb::Indices indices_of(const void* ptr, int index_type, long long count, const char* what) {
+  require(index_type == PS_I32 || index_type == PS_I64, what, "the index type is PS_I32 or PS_I64");
+  require(count >= 0 && count <= 0x7fffffffLL, what, "the number of indices must be in [0, 2^31)");
+  require(ptr != nullptr || count == 0, what, "null buffer");
+  require(reinterpret_cast<uintptr_t>(ptr) % (index_type == PS_I64 ? 8 : 4) == 0, what, "the indices are not aligned to their type");
+  return {ptr, index_type == PS_I64, count};
+}
+
+void require_experts(int tokens, int experts, int top_k, const char* what) {
+  require(tokens >= 0, what, "the number of tokens must be >= 0");
+  require(experts >= 1 && experts <= psb::kMaxExperts, what, "the number of experts must be in [1, 1024]");
+  require(top_k >= 1 && top_k <= psb::kMaxTopK, what, "top_k must be in [1, 32]");
+  require((long long)tokens * top_k <= 0x7fffffffLL, what, "tokens * top_k must be below 2^31");
 }
 
 }  // namespace
@@ -253,6 +293,142 @@ int ps_sddmm_csr(const ps_matrix* h, int N, const float* lhs, const float* rhs, 
     const psb::Matrix& m = M(h);
     require_device(m);
     psb::sddmm_csr_launch(m, N, lhs, rhs, out, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ps_embedding(const void* table, int dtype, long long rows, int width, long long table_stride, const void* tokens,
+                 int index_type, long long n, float scale, void* out, long long out_stride, void* stream) {
+  return guarded([&] {
+    const char* what = "ps_embedding";
+    const int size = size_of(dtype, what);
+    const psb::Indices index = indices_of(tokens, index_type, n, what);
+    require(rows >= 1, what, "the table has no rows");
+    require_rows(table, table_stride, rows, width, size, what);
+    require_rows(out, out_stride, n, width, size, what);
+    psb::embedding_launch(dtype, {table, table_stride}, rows, width, index, scale, {out, out_stride},
+                          static_cast<cudaStream_t>(stream));
+  });
+}
+
+long long ps_embedding_grad_workspace(long long n, long long rows, int width) {
+  if (n < 0 || n > 0x7fffffffLL || rows < 1 || rows >= 0x7fffffffLL || width < 1 || width > (1 << 24)) return -1;
+  return (long long)psb::embedding_grad_workspace(n, rows, width);
+}
+
+int ps_embedding_grad(const void* grad, int grad_dtype, long long grad_stride, const void* tokens, int index_type, long long n,
+                      float scale, long long padding, int accumulate, void* grad_table, int table_dtype, long long table_stride,
+                      long long rows, int width, void* workspace, long long workspace_bytes, void* stream) {
+  return guarded([&] {
+    const char* what = "ps_embedding_grad";
+    const int in_size = size_of(grad_dtype, what), out_size = size_of(table_dtype, what);
+    require(table_dtype == grad_dtype || table_dtype == PS_F32, what, "the table's gradient has the type of grad or PS_F32");
+    const psb::Indices index = indices_of(tokens, index_type, n, what);
+    require(rows >= 1 && rows < 0x7fffffffLL, what, "the table's rows must be in [1, 2^31 - 2]");
+    require_rows(grad, grad_stride, n, width, in_size, what);
+    require_rows(grad_table, table_stride, rows, width, out_size, what);
+    require(workspace_bytes >= (long long)psb::embedding_grad_workspace(n, rows, width) && workspace != nullptr, what,
+            "the workspace is smaller than ps_embedding_grad_workspace says");
+    require(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, what, "the workspace must begin at a multiple of 256 bytes");
+    psb::embedding_grad_launch(grad_dtype, {grad, grad_stride}, index, scale, padding, accumulate != 0, table_dtype,
+                               {grad_table, table_stride}, rows, width, workspace, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ps_route(const void* logits, int dtype, long long logits_stride, int tokens, int experts, int top_k, int normalize,
+             float* weights, int* chosen, void* stream) {
+  return guarded([&] {
+    const char* what = "ps_route";
+    const int size = size_of(dtype, what);
+    require_experts(tokens, experts, top_k, what);
+    require(top_k <= experts, what, "top_k is larger than the number of experts");
+    require_rows(logits, logits_stride, tokens, experts, size, what);
+    require_array(weights, tokens, what);
+    require_array(chosen, tokens, what);
+    psb::route_launch(dtype, {logits, logits_stride}, tokens, experts, top_k, normalize != 0, weights, chosen,
+                      static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ps_route_grad(const float* grad_weights, const void* logits, int dtype, long long logits_stride, const float* weights,
+                  const int* chosen, int tokens, int experts, int top_k, int normalize, void* grad_logits,
+                  long long grad_logits_stride, void* stream) {
+  return guarded([&] {
+    const char* what = "ps_route_grad";
+    const int size = size_of(dtype, what);
+    require_experts(tokens, experts, top_k, what);
+    require(top_k <= experts, what, "top_k is larger than the number of experts");
+    require_rows(logits, logits_stride, tokens, experts, size, what);
+    require_rows(grad_logits, grad_logits_stride, tokens, experts, size, what);
+    require_array(grad_weights, tokens, what);
+    require_array(weights, tokens, what);
+    require_array(chosen, tokens, what);
+    psb::route_grad_launch(dtype, grad_weights, {logits, logits_stride}, weights, chosen, tokens, experts, top_k, normalize != 0,
+                           {grad_logits, grad_logits_stride}, static_cast<cudaStream_t>(stream));
+  });
+}
+
+long long ps_dispatch_rows(long long slots, int experts, int align) {
+  if (slots < 0 || slots > 0x7fffffffLL || experts < 1 || align < 1) return -1;
+  return psb::dispatch_rows(slots, experts, align);
+}
+
+int ps_dispatch(const void* x, int dtype, long long x_stride, const void* chosen, int index_type, int tokens, int top_k,
+                int experts, int align, int width, void* rows, long long rows_stride, long long row_count, int zero_tail,
+                int* position, int* offsets, int* counts, void* stream) {
+  return guarded([&] {
+    const char* what = "ps_dispatch";
+    const int size = size_of(dtype, what);
+    require_experts(tokens, experts, top_k, what);
+    require(align >= 1 && align <= 65536, what, "align must be in [1, 65536]");
+    const long long slots = (long long)tokens * top_k, need = psb::dispatch_rows(slots, experts, align);
+    const psb::Indices index = indices_of(chosen, index_type, slots, what);
+    require(need <= 0x7fffffffLL, what, "the rows in expert order must be below 2^31");
+    require(row_count >= need, what, "fewer rows than ps_dispatch_rows says");
+    require_rows(x, x_stride, tokens, width, size, what);
+    require_rows(rows, rows_stride, row_count, width, size, what);
+    require_array(position, slots, what);
+    require_array(offsets, experts, what);
+    require_array(counts, experts, what);
+    psb::dispatch_launch(dtype, {x, x_stride}, index, tokens, top_k, experts, align, width, {rows, rows_stride}, row_count,
+                         zero_tail != 0, position, offsets, counts, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ps_combine(const void* y, int dtype, long long y_stride, long long row_count, const int* position, const float* weights,
+               const void* add, long long add_stride, int tokens, int top_k, int width, void* out, long long out_stride,
+               void* stream) {
+  return guarded([&] {
+    const char* what = "ps_combine";
+    const int size = size_of(dtype, what);
+    require_experts(tokens, 1, top_k, what);
+    require_rows(y, y_stride, row_count, width, size, what);
+    require_rows(out, out_stride, tokens, width, size, what);
+    if (add) require_rows(add, add_stride, tokens, width, size, what);
+    require_array(position, tokens, what);
+    if (weights) require_array(weights, tokens, what);
+    psb::combine_launch(dtype, {y, y_stride}, row_count, position, weights, {add, add_stride}, tokens, top_k, width,
+                        {out, out_stride}, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ps_combine_grad(const void* grad, int dtype, long long grad_stride, const void* y, long long y_stride, long long row_count,
+                    const int* position, const int* offsets, const int* counts, int experts, const float* weights, int tokens,
+                    int top_k, int width, void* grad_y, long long grad_y_stride, int zero_tail, float* grad_weights, void* stream) {
+  return guarded([&] {
+    const char* what = "ps_combine_grad";
+    const int size = size_of(dtype, what);
+    require_experts(tokens, experts, top_k, what);
+    require_rows(grad, grad_stride, tokens, width, size, what);
+    require_rows(y, y_stride, row_count, width, size, what);
+    require_rows(grad_y, grad_y_stride, row_count, width, size, what);
+    require_array(position, tokens, what);
+    require_array(offsets, experts, what);
+    require_array(counts, experts, what);
+    require_array(weights, tokens, what);
+    require_array(grad_weights, tokens, what);
+    psb::combine_grad_launch(dtype, {grad, grad_stride}, {y, y_stride}, row_count, position, offsets, counts, experts, weights,
+                             tokens, top_k, width, {grad_y, grad_y_stride}, zero_tail != 0, grad_weights,
+                             static_cast<cudaStream_t>(stream));
   });
 }
 

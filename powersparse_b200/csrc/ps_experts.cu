@@ -1,0 +1,498 @@
+// A mixture layer's index operators: the router's softmax and top-k, the tokens'
+// rows in the order of their experts, the experts' rows back with their weights, and
+// the gradients of all three.
+//
+// With the slot (t, j) of token t's j-th expert and its row position(t, j) in expert
+// order:
+//
+//   dispatch      rows[position(t, j), :] = x[t, :]
+//   combine       out[t, :] = add[t, :] + sum_j w[t, j] * y[position(t, j), :]
+//   combine_grad  grad_y[position(t, j), :] = w[t, j] * g[t, :]
+//                 grad_w[t, j] = <g[t, :], y[position(t, j), :]>
+//
+// combine is the SpMM of the matrix with w[t, j] at (t, position(t, j)), the gradient
+// of its values is that matrix's SDDMM, and dispatch is the transposed SpMM of ones;
+// the matrix is new in every call and has at most top_k elements a row and one a
+// column, so every kernel here walks tokens and no sum needs atomics.
+#include "ps_index_sort.cuh"
+#include "ps_rows.cuh"
+
+namespace psb {
+namespace {
+
+// ---- router -----------------------------------------------------------------------
+// A warp a token, E / 32 scores a lane in registers.  Scores compare as integers that
+// keep the order of the numbers (-0 as +0); of equal scores the lowest index comes
+// first.  A score of -inf switches an expert off: it is never chosen.
+constexpr int kRouteWarps = 8;
+
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_scores(const T* row, int experts, float (&x)[V]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 32 + lane;
+    x[v] = e < experts ? to_float(row[e]) : -INFINITY;
+  }
+}
+
+// Largest score of the row (0 where all are -inf, so that x - max is not NaN), and
+// the sum of exp(x - max) over the row.
+template <int V>
+__device__ __forceinline__ void row_softmax(const float (&x)[V], float& top, float& sum) {
+  top = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < V; ++v) top = fmaxf(top, x[v]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (top == -INFINITY) top = 0.f;
+  sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum += expf(x[v] - top);
+  sum = warp_sum(sum);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* __restrict__ logits, long long stride, int tokens,
+                                                                 int experts, int top_k, bool normalize,
+                                                                 float* __restrict__ weights, int* __restrict__ chosen) {
+  const int lane = threadIdx.x & 31;
+  const long long t = blockIdx.x * (long long)kRouteWarps + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  float x[V];
+  load_scores<T, V>(logits + t * stride, experts, x);
+  float top, sum;
+  row_softmax<V>(x, top, sum);
+  bool nan = false;
+  uint32_t key[V];  // 0: off, or taken already
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    nan = nan || x[v] != x[v];
+    key[v] = x[v] > -INFINITY ? ordered(x[v]) : 0u;  // a NaN compares false
+  }
+  nan = __any_sync(0xffffffffu, nan);
+  int mine = -1;        // lane j: the j-th choice
+  float e_mine = 0.f;   // and its exp(x - top)
+  for (int j = 0; j < top_k; ++j) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) best = max(best, key[v]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    if (best == 0) break;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v)
+      if (key[v] == best) at = v * 32 + lane;
+    at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (at == v * 32 + lane) key[v] = 0;
+    if (lane == j) {
+      mine = at;
+      const uint32_t bits = best & 0x80000000u ? best & 0x7fffffffu : ~best;
+      e_mine = expf(__uint_as_float(bits) - top);
+    }
+  }
+  const float total = normalize ? warp_sum(e_mine) : sum;
+  if (lane < top_k) {
+    weights[t * top_k + lane] = mine < 0 ? 0.f : nan ? NAN : e_mine / total;
+    chosen[t * top_k + lane] = mine;
+  }
+}
+
+// With p the softmax that the weights are shares of, and G = sum_j g_j w_j:
+//   d logits[e] = p[e] * (g of the choice e, or 0) - p[e] * G.
+// Shares of all experts: p from the logits, dense.  Shares of the chosen ones
+// (normalize): p is the weights, zero elsewhere, and the logits are not read.
+template <typename T, int V, bool kNormalize>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const float* __restrict__ grad, const T* __restrict__ logits,
+                                                                      long long stride, const float* __restrict__ weights,
+                                                                      const int* __restrict__ chosen, int tokens, int experts,
+                                                                      int top_k, T* __restrict__ out, long long out_stride) {
+  const int lane = threadIdx.x & 31;
+  const long long t = blockIdx.x * (long long)kRouteWarps + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  int mine = -1;
+  float g = 0.f, w = 0.f;
+  if (lane < top_k) {
+    mine = chosen[t * top_k + lane];
+    if (mine >= 0 && mine < experts) {
+      g = grad[t * top_k + lane];
+      w = weights[t * top_k + lane];
+    } else {
+      mine = -1;
+    }
+  }
+  const float inner = warp_sum(g * w);
+  float p[V], d[V];
+  if (!kNormalize) {
+    float top, sum;
+    load_scores<T, V>(logits + t * stride, experts, p);
+    row_softmax<V>(p, top, sum);
+    const float inv = sum > 0.f ? 1.f / sum : sum;  // a NaN stays
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] = expf(p[v] - top) * inv;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) d[v] = kNormalize ? 0.f : -p[v] * inner;
+  for (int j = 0; j < top_k; ++j) {
+    const int e = __shfl_sync(0xffffffffu, mine, j);
+    const float gj = __shfl_sync(0xffffffffu, g, j), wj = __shfl_sync(0xffffffffu, w, j);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (e == v * 32 + lane) d[v] += kNormalize ? wj * (gj - inner) : p[v] * gj;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 32 + lane;
+    if (e < experts) out[t * out_stride + e] = from_float<T>(d[v]);
+  }
+}
+
+// ---- order of the slots by expert ---------------------------------------------------
+__global__ void __launch_bounds__(kSortThreads) expert_order(const void* __restrict__ chosen, bool wide, long long n, int experts,
+                                                             int align, int* __restrict__ position, int* __restrict__ offsets,
+                                                             int* __restrict__ counts) {
+  extern __shared__ uint32_t smem[];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  const SortShared sh(smem, experts);
+  const Strip strip = warp_strip(n, rank, blocks);
+  auto digit = [&](long long i) {
+    const long long e = index_at(chosen, wide, i);
+    return e >= 0 && e < experts ? int(e) : -1;
+  };
+  auto widen = [&](uint32_t count) { return (count + uint32_t(align) - 1) / uint32_t(align) * uint32_t(align); };
+  digit_positions(sh, experts, strip, digit, widen, [&](int e, uint32_t begin, uint32_t count) {
+    if (rank != 0) return;
+    offsets[e] = int(begin);
+    counts[e] = int(count);
+    if (e == experts - 1) offsets[experts] = int(begin + widen(count));
+  });
+  place_digits(strip, sh.rows + (threadIdx.x >> 5) * experts, digit,
+               [&](long long i, int d, uint32_t p) { position[i] = d < 0 ? -1 : int(p); });
+}
+
+// ---- rows -----------------------------------------------------------------------
+// The blocks that write the rows without a token come first: `tail` blocks for the
+// rows behind the last expert, then `pad` blocks, kPadBlocks an expert, for the rows
+// between an expert's tokens and the next expert.  Then the tokens' blocks:
+// 2^lanes_log2 threads a token.
+constexpr int kRowThreads = 256;
+constexpr int kRowUnroll = 4;
+constexpr int kPadBlocks = 8;
+constexpr int kTailBlocks = 512;
+
+struct Blanks {
+  const int* offsets;
+  const int* counts;
+  long long rows;
+  int experts, tail, pad;
+  __host__ __device__ int blocks() const { return tail + pad; }
+};
+
+// Block blockIdx.x < b.blocks() of the rows without a token.  The bounds hold whatever
+// the plan's arrays say.
+template <int B>
+__device__ __forceinline__ void zero_blanks(const Blanks& b, int words, unsigned char* out, long long out_bytes) {
+  constexpr int kWarps = kRowThreads / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  long long begin, end = b.rows;
+  int part = blockIdx.x, parts = b.tail;
+  if (part < b.tail) {
+    begin = b.offsets[b.experts];
+  } else {
+    const int e = (part - b.tail) / kPadBlocks;
+    part = (part - b.tail) % kPadBlocks;
+    parts = kPadBlocks;
+    begin = (long long)b.offsets[e] + b.counts[e];
+    end = min((long long)b.offsets[e + 1], b.rows);
+  }
+  for (long long r = max(0LL, begin) + part * kWarps + warp; r < end; r += parts * kWarps)
+    for (int c = lane; c < words; c += 32) reinterpret_cast<Word<B>*>(out + r * out_bytes)[c] = Word<B>{};
+}
+
+template <int B>
+__global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsigned char* __restrict__ x, long long x_bytes,
+                                                                    const int* __restrict__ position, Blanks blanks, int tokens,
+                                                                    int top_k, int words, unsigned char* __restrict__ out,
+                                                                    long long out_bytes, int lanes_log2) {
+  if (int(blockIdx.x) < blanks.blocks()) return zero_blanks<B>(blanks, words, out, out_bytes);
+  const long long rows = blanks.rows;
+  const int lanes = 1 << lanes_log2;
+  const long long t = (blockIdx.x - blanks.blocks()) * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  if (t >= tokens) return;
+  const auto* src = reinterpret_cast<const Word<B>*>(x + t * x_bytes);
+  for (int c = threadIdx.x & (lanes - 1); c < words; c += lanes * kRowUnroll) {
+    Word<B> v[kRowUnroll];
+#pragma unroll
+    for (int u = 0; u < kRowUnroll; ++u)
+      if (c + u * lanes < words) v[u] = __ldg(src + c + u * lanes);
+    for (int j = 0; j < top_k; ++j) {
+      const int p = position[t * top_k + j];
+      if (p < 0 || p >= rows) continue;
+      auto* dst = reinterpret_cast<Word<B>*>(out + p * out_bytes);
+#pragma unroll
+      for (int u = 0; u < kRowUnroll; ++u)
+        if (c + u * lanes < words) dst[c + u * lanes] = v[u];
+    }
+  }
+}
+
+template <typename T, int N, bool kWeighted>
+__global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict__ y, long long y_stride, long long rows,
+                                                            const int* __restrict__ position, const float* __restrict__ weights,
+                                                            const T* add, long long add_stride, int tokens, int top_k, int width,
+                                                            T* out, long long out_stride, int lanes_log2) {
+  constexpr int kSlots = 4;  // rows in flight
+  const int lanes = 1 << lanes_log2;
+  const long long t = blockIdx.x * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  if (t >= tokens) return;
+  for (int c = (threadIdx.x & (lanes - 1)) * N; c < width; c += lanes * N) {
+    float acc[N];
+    if (add) {
+      Pack<T, N> a;
+      a.load_rw(add + t * add_stride + c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] = a.get(e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] = 0.f;
+    }
+    for (int j0 = 0; j0 < top_k; j0 += kSlots) {
+      Pack<T, N> v[kSlots];
+      float w[kSlots];
+      bool on[kSlots];
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) {
+        const int p = j0 + s < top_k ? position[t * top_k + j0 + s] : -1;
+        on[s] = p >= 0 && p < rows;
+        if (on[s]) {
+          v[s].load(y + p * y_stride + c);
+          w[s] = kWeighted ? weights[t * top_k + j0 + s] : 1.f;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s)
+        if (on[s]) {
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[e] += w[s] * v[s].get(e);
+        }
+    }
+    Pack<T, N> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o.set(e, acc[e]);
+    o.store(out + t * out_stride + c);
+  }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kRowThreads) combine_grad_rows(const T* __restrict__ grad, long long grad_stride,
+                                                                 const T* __restrict__ y, long long y_stride,
+                                                                 const int* __restrict__ position, Blanks blanks,
+                                                                 const float* __restrict__ weights, int tokens, int top_k,
+                                                                 int width, T* __restrict__ grad_y, long long grad_y_stride,
+                                                                 float* __restrict__ grad_weights, int lanes_log2) {
+  constexpr int kSlots = 8;  // rows in flight, and dot products held
+  constexpr int kBytes = N * int(sizeof(T));
+  if (int(blockIdx.x) < blanks.blocks())
+    return zero_blanks<kBytes>(blanks, width / N, reinterpret_cast<unsigned char*>(grad_y), grad_y_stride * (long long)sizeof(T));
+  const long long rows = blanks.rows;
+  __shared__ float parts[kRowThreads / 32][kSlots];
+  const int lanes = 1 << lanes_log2;  // 32 at least
+  const long long t = (blockIdx.x - blanks.blocks()) * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  const bool live = t < tokens;  // the whole warp; the others take part in the block's barriers
+  for (int j0 = 0; j0 < top_k; j0 += kSlots) {
+    float dot[kSlots], w[kSlots];
+    int p[kSlots];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      const bool slot = live && j0 + s < top_k;
+      p[s] = slot ? position[t * top_k + j0 + s] : -1;
+      if (p[s] >= rows) p[s] = -1;
+      w[s] = p[s] >= 0 ? weights[t * top_k + j0 + s] : 0.f;
+      dot[s] = 0.f;
+    }
+    if (live) {
+      for (int c = (threadIdx.x & (lanes - 1)) * N; c < width; c += lanes * N) {
+        Pack<T, N> g, v[kSlots];
+        g.load(grad + t * grad_stride + c);
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s)
+          if (p[s] >= 0) v[s].load(y + p[s] * y_stride + c);
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s) {
+          if (p[s] < 0) continue;
+          Pack<T, N> o;
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            dot[s] += g.get(e) * v[s].get(e);
+            o.set(e, w[s] * g.get(e));
+          }
+          o.store(grad_y + p[s] * grad_y_stride + c);
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) dot[s] = warp_sum(dot[s]);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = lanes >> 5;
+    if (warps > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s)
+        if (lane == s) parts[warp][s] = dot[s];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+      if (lane == s && live && j0 + s < top_k && warp % warps == 0) {
+        float sum = dot[s];
+        for (int k = 1; k < warps; ++k) sum += parts[warp + k][s];
+        grad_weights[t * top_k + j0 + s] = p[s] >= 0 ? sum : 0.f;
+      }
+  }
+}
+
+template <int N>
+struct Count {
+  static constexpr int value = N;
+};
+
+// f(V constant) with 32 * V >= experts.
+template <typename F>
+void with_scores(int experts, F&& f) {
+  if (experts <= 32) f(Count<1>());
+  else if (experts <= 64) f(Count<2>());
+  else if (experts <= 128) f(Count<4>());
+  else if (experts <= 256) f(Count<8>());
+  else if (experts <= 512) f(Count<16>());
+  else f(Count<32>());
+}
+
+// log2 of the threads that share a row of `words` words, `each` of them a thread.
+int row_lanes(int words, int each, int least_log2) {
+  return std::min(8, std::max(least_log2, log2_up(ceil_div(words, each))));
+}
+
+int tail_blocks(bool zero_tail, long long rows) {
+  return zero_tail ? int(std::min<long long>(kTailBlocks, ceil_div_ll(rows, kRowThreads / 32))) : 0;
+}
+
+}  // namespace
+
+void route_launch(int dtype, RowsIn logits, int tokens, int experts, int top_k, bool normalize, float* weights, int* chosen,
+                  cudaStream_t stream) {
+  if (tokens == 0) return;
+  with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    with_scores(experts, [&](auto v) {
+      route_tokens<T, decltype(v)::value><<<ceil_div(tokens, kRouteWarps), kRouteWarps * 32, 0, stream>>>(
+          static_cast<const T*>(logits.ptr), logits.stride, tokens, experts, top_k, normalize, weights, chosen);
+    });
+  });
+  PSB_LAUNCH_CHECK();
+}
+
+void route_grad_launch(int dtype, const float* grad_weights, RowsIn logits, const float* weights, const int* chosen, int tokens,
+                       int experts, int top_k, bool normalize, RowsOut grad_logits, cudaStream_t stream) {
+  if (tokens == 0) return;
+  with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    with_scores(experts, [&](auto v) {
+      constexpr int V = decltype(v)::value;
+      auto kernel = normalize ? route_grad_tokens<T, V, true> : route_grad_tokens<T, V, false>;
+      kernel<<<ceil_div(tokens, kRouteWarps), kRouteWarps * 32, 0, stream>>>(
+          grad_weights, static_cast<const T*>(logits.ptr), logits.stride, weights, chosen, tokens, experts, top_k,
+          static_cast<T*>(grad_logits.ptr), grad_logits.stride);
+    });
+  });
+  PSB_LAUNCH_CHECK();
+}
+
+long long dispatch_rows(long long slots, int experts, int align) {
+  return (slots + std::min<long long>(experts, slots) * (align - 1)) / align * align;
+}
+
+void dispatch_launch(int dtype, RowsIn x, Indices chosen, int tokens, int top_k, int experts, int align, int width, RowsOut out,
+                     long long row_count, bool zero_tail, int* position, int* offsets, int* counts, cudaStream_t stream) {
+  const long long n = chosen.count;
+  launch_cluster(expert_order, sort_blocks(n), sort_smem(experts), stream, chosen.ptr, chosen.wide, n, experts, align, position,
+                 offsets, counts);
+  const Blanks blanks{offsets, counts, row_count, experts, tail_blocks(zero_tail, row_count), align > 1 ? experts * kPadBlocks : 0};
+  if (n == 0 && blanks.tail == 0) return;
+  const int size = dtype_size(dtype);
+  const long long row_bytes = (long long)width * size;
+  auto run = [&](auto bytes) {
+    constexpr int B = decltype(bytes)::value;
+    const int words = int(row_bytes / B), lanes_log2 = row_lanes(words, kRowUnroll, 0);
+    const unsigned blocks = grid_x(blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2));
+    dispatch_rows_kernel<B><<<blocks, kRowThreads, 0, stream>>>(
+        static_cast<const unsigned char*>(x.ptr), x.stride * size, position, blanks, tokens, top_k, words,
+        static_cast<unsigned char*>(out.ptr), out.stride * size, lanes_log2);
+  };
+  auto fits = [&](int bytes) {
+    return row_bytes % bytes == 0 && rows_aligned(x.ptr, x.stride, size, bytes) && rows_aligned(out.ptr, out.stride, size, bytes);
+  };
+  if (fits(16)) run(Count<16>());
+  else if (fits(4)) run(Count<4>());
+  else run(Count<2>());
+  PSB_LAUNCH_CHECK();
+}
+
+void combine_launch(int dtype, RowsIn y, long long rows, const int* position, const float* weights, RowsIn add, int tokens,
+                    int top_k, int width, RowsOut out, cudaStream_t stream) {
+  if (tokens == 0) return;
+  const int size = dtype_size(dtype);
+  with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    auto run = [&](auto per) {
+      constexpr int N = decltype(per)::value;
+      const int lanes_log2 = row_lanes(ceil_div(width, N), 2, 0);
+      const unsigned blocks = grid_x(ceil_div_ll(tokens, kRowThreads >> lanes_log2));
+      auto kernel = weights ? combine_rows<T, N, true> : combine_rows<T, N, false>;
+      kernel<<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(y.ptr), y.stride, rows, position, weights,
+                                                 static_cast<const T*>(add.ptr), add.stride, tokens, top_k, width,
+                                                 static_cast<T*>(out.ptr), out.stride, lanes_log2);
+    };
+    constexpr int kWide = 16 / sizeof(T);
+    if (width % kWide == 0 && rows_aligned(y.ptr, y.stride, size, 16) && rows_aligned(out.ptr, out.stride, size, 16) &&
+        (!add.ptr || rows_aligned(add.ptr, add.stride, size, 16)))
+      run(Count<kWide>());
+    else
+      run(Count<1>());
+  });
+  PSB_LAUNCH_CHECK();
+}
+
+void combine_grad_launch(int dtype, RowsIn grad, RowsIn y, long long rows, const int* position, const int* offsets,
+                         const int* counts, int experts, const float* weights, int tokens, int top_k, int width, RowsOut grad_y,
+                         bool zero_tail, float* grad_weights, cudaStream_t stream) {
+  const Blanks blanks{offsets, counts, rows, experts, tail_blocks(zero_tail, rows), experts * kPadBlocks};
+  const int size = dtype_size(dtype);
+  with_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    auto run = [&](auto per) {
+      constexpr int N = decltype(per)::value;
+      const int lanes_log2 = row_lanes(ceil_div(width, N), 8, 5);
+      const unsigned blocks = grid_x(blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2));
+      combine_grad_rows<T, N><<<blocks, kRowThreads, 0, stream>>>(
+          static_cast<const T*>(grad.ptr), grad.stride, static_cast<const T*>(y.ptr), y.stride, position, blanks,
+          weights, tokens, top_k, width, static_cast<T*>(grad_y.ptr), grad_y.stride, grad_weights, lanes_log2);
+    };
+    constexpr int kWide = 16 / sizeof(T);
+    if (width % kWide == 0 && rows_aligned(grad.ptr, grad.stride, size, 16) && rows_aligned(y.ptr, y.stride, size, 16) &&
+        rows_aligned(grad_y.ptr, grad_y.stride, size, 16))
+      run(Count<kWide>());
+    else
+      run(Count<1>());
+  });
+  PSB_LAUNCH_CHECK();
+}
+
+}  // namespace psb

@@ -1,0 +1,646 @@
+"""GPU tests: the operators on rows chosen by an index against their formulas in 64 bits.
+
+Tolerances count roundings.  u = 2^-24 is half a step of FP32, half(T) half a step of the
+stored type relative to the value (finfo.eps / 2), tiny(T) half of its smallest
+subnormal.  A sum of m terms in FP32, in whatever order, is off by at most
+m * u * sum |terms| to first order (products included); the factor 1.01 covers the
+higher orders (m * u < 1e-2 in every test).
+"""
+import math
+
+import pytest
+import torch
+
+import powersparse_b200 as psb
+import powersparse_b200.torch_ops  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+U = 2.0 ** -24
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def check(got, want, slack=0.0, tag=""):
+    """|got - want| <= half a step of got's type at want + slack (the FP32 part, absolute)."""
+    assert got.shape == want.shape and want.dtype == torch.float64
+    got64 = got.double()
+    room = 1.01 * (want.abs() * half(got.dtype) + slack * (1 + half(got.dtype))) + tiny(got.dtype)
+    bad = ~((got64 - want).abs() <= room)
+    assert not bad.any(), (tag, int(bad.sum()), bad.nonzero()[:3].tolist(), got64[bad][:3].tolist(), want[bad][:3].tolist())
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32):
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def strided(t, extra, offset=0):
+    """t's values in a tensor whose rows are `extra` elements further apart, begun at element `offset`."""
+    rows, width = t.shape
+    buf = torch.full((rows * (width + extra) + offset + 1,), math.nan, device="cuda", dtype=t.dtype)
+    view = buf[offset: offset + rows * (width + extra)].view(rows, width + extra)[:, :width]
+    view.copy_(t)
+    return view
+
+
+# ------------------------------------------------------------------------------------ embedding
+
+WIDTHS = [1, 2, 7, 8, 33, 128, 515, 1024, 4104]
+
+
+def embedding64(table, tokens, scale):
+    t = tokens.reshape(-1).long()
+    inside = (t >= 0) & (t < table.shape[0])
+    out = table.double()[t.clamp(0, table.shape[0] - 1)] * scale
+    return out.masked_fill(~inside[:, None], 0.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", WIDTHS)
+def test_embedding(dtype, width):
+    g = gen(width)
+    for n, rows, index in ((1, 1, torch.int64), (5, 3, torch.int32), (257, 1000, torch.int64)):
+        table = randn(g, rows, width, dtype=dtype)
+        tokens = torch.randint(-2, rows + 2, (n,), generator=g, device="cuda").to(index)
+        scale = 22.5
+        want = embedding64(table, tokens, torch.tensor(scale, dtype=F32).double().item())
+        check(psb.embedding(table, tokens, scale), want, want.abs() * U)
+        assert torch.equal(psb.embedding(table, tokens).double(), embedding64(table, tokens, 1.0))  # a copy is exact
+        out = strided(torch.zeros(n, width, device="cuda", dtype=dtype), 3)
+        psb.embedding(strided(table, 5, 1), tokens, scale, out=out)
+        check(out, want, want.abs() * U)
+
+
+def test_embedding_shapes_and_far_tokens():
+    table = randn(gen(0), 10, 24, dtype=BF16)
+    tokens = torch.tensor([[0, 9, 2**40], [-2**40, 2**32 + 1, 3]], device="cuda")  # 2^32 + 1 is not row 1
+    out = psb.embedding(table, tokens)
+    assert out.shape == (2, 3, 24)
+    assert torch.equal(out.view(6, 24).double(), embedding64(table, tokens, 1.0))
+    assert psb.embedding(table, tokens[:0]).shape == (0, 3, 24)
+    # What stands in rows that no token names has no effect, inf and NaN included.
+    table[1:3] = math.nan
+    table[5] = math.inf
+    assert torch.equal(psb.embedding(table, tokens).view(6, 24)[[0, 1, 5]], table[[0, 9, 3]])
+    assert not psb.embedding(table, tokens).isnan().any()
+
+
+def test_embedding_offsets_pass_32_bits():
+    rows, width = 600_000, 4096  # 2.4e9 elements
+    table = torch.empty(rows, width, device="cuda", dtype=BF16)
+    tokens = torch.tensor([0, rows - 1, 524_288, 524_287, rows], device="cuda")
+    for i, t in enumerate(tokens[:-1].tolist()):
+        table[t] = i + 1
+    out = psb.embedding(table, tokens)
+    assert out.double().mean(1).tolist() == [1, 2, 3, 4, 0]
+    grad = torch.ones(5, width, device="cuda", dtype=BF16)
+    psb.embedding_grad(grad, tokens, rows, out=table, scale=3.0)
+    assert table[tokens[:-1]].double().mean(1).tolist() == [3, 3, 3, 3]
+    assert table.count_nonzero().item() == 4 * width
+
+
+def grad64(grad, tokens, rows, scale, padding=None):
+    t = tokens.reshape(-1).long()
+    on = (t >= 0) & (t < rows) & (t != (-1 if padding is None else padding))
+    g = grad.double()[on] * scale
+    out = torch.zeros(rows, grad.shape[1], dtype=torch.float64, device="cuda").index_add_(0, t[on], g)
+    size = torch.zeros_like(out).index_add_(0, t[on], g.abs())
+    many = torch.zeros(rows, dtype=torch.float64, device="cuda").index_add_(0, t[on], torch.ones_like(t[on], dtype=torch.float64))
+    return out, size * (many[:, None] + 2) * U
+
+
+def batch(g, kind, n, rows, index=torch.int64):
+    if kind == "one":
+        t = torch.full((n,), rows // 2, device="cuda")
+    elif kind == "empty":
+        t = torch.full((n,), -1, device="cuda")
+    elif kind == "skewed":
+        t = (rows ** torch.rand(n, generator=g, device="cuda")).long() - 1
+    elif kind == "distinct":
+        t = torch.randperm(rows, generator=g, device="cuda")[:n]
+    elif kind == "sorted":
+        t = torch.arange(n, device="cuda") * rows // max(n, 1)
+    else:
+        t = torch.randint(-3, rows + 3, (n,), generator=g, device="cuda")
+    return t.to(index)
+
+
+@pytest.mark.parametrize("dtype,out", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+@pytest.mark.parametrize("width", [1, 8, 33, 128, 515, 1032])
+def test_embedding_grad(dtype, out, width):
+    g = gen(width)
+    for kind, n, rows, index in (("any", 1, 1, torch.int32), ("any", 3, 7, torch.int64), ("skewed", 333, 50, torch.int32),
+                                 ("distinct", 200, 257, torch.int64), ("one", 1000, 300, torch.int64), ("empty", 64, 20, torch.int32),
+                                 ("skewed", 5000, 3000, torch.int64), ("sorted", 4097, 100, torch.int32)):
+        tokens, grad = batch(g, kind, n, rows, index), randn(g, n, width, dtype=dtype)
+        want, slack = grad64(grad, tokens, rows, 0.75)
+        check(psb.embedding_grad(grad, tokens, rows, 0.75, dtype=out), want, slack, (kind, n, rows))
+        dst = strided(torch.full((rows, width), 7.0, device="cuda", dtype=out), 2, 1)
+        psb.embedding_grad(strided(grad, 3), tokens, rows, 0.75, out=dst)
+        check(dst, want, slack, (kind, "strided"))
+
+
+@pytest.mark.parametrize("kind", ["any", "skewed", "one", "distinct", "sorted", "empty"])
+@pytest.mark.parametrize("n,rows", [(20000, 40000), (70001, 70001), (16384, 1025), (40000, 2_000_000), (9000, 512), (2049, 1023)])
+def test_embedding_grad_order_of_large_batches(kind, n, rows):
+    g = gen(n + rows)
+    if kind == "distinct" and n > rows:
+        n = rows
+    tokens, grad = batch(g, kind, n, rows), randn(g, n, 16, dtype=BF16)
+    want, slack = grad64(grad, tokens, rows, 1.0)
+    got = psb.embedding_grad(grad, tokens, rows, dtype=F32)
+    check(got, want, slack)
+    assert torch.equal(got, psb.embedding_grad(grad, tokens, rows, dtype=F32))  # the same bits again
+
+
+def test_embedding_grad_of_a_million_tokens_and_many_passes():
+    g = gen(5)
+    n, rows = 1_100_000, 5_000_000
+    tokens, grad = batch(g, "skewed", n, rows), randn(g, n, 4)
+    want, slack = grad64(grad, tokens, rows, 1.0)
+    check(psb.embedding_grad(grad, tokens, rows), want, slack)
+    rows = 2**31 - 2  # four digit passes; the sums go to the rows that occur, the others stay untouched
+    tokens = torch.tensor([3, 7, 3, 2**20, 7, 3, -1, 2**31 - 2, 2**31], device="cuda")
+    out = torch.zeros(2**20 + 1, 8, device="cuda")
+    lib = psb.load_library()
+    ws = torch.empty(lib.ps_embedding_grad_workspace(9, rows, 8), dtype=torch.uint8, device="cuda")
+    grad = randn(g, 9, 8)
+    s = torch.cuda.current_stream().cuda_stream
+    assert lib.ps_embedding_grad(grad.data_ptr(), 0, 8, tokens.data_ptr(), 1, 9, 1.0, -1, 1, out.data_ptr(), 0, 8, rows, 8,
+                                 ws.data_ptr(), ws.numel(), s) == psb.PS_OK
+    want, slack = grad64(grad, tokens, 2**20 + 1, 1.0)
+    check(out, want, slack)
+
+
+def test_embedding_grad_padding_accumulate_and_no_tokens():
+    g = gen(9)
+    tokens, grad = batch(g, "skewed", 3000, 100), randn(g, 3000, 40, dtype=BF16)
+    want, slack = grad64(grad, tokens, 100, 2.0, padding=0)
+    out = psb.embedding_grad(grad, tokens, 100, 2.0, padding=0, dtype=F32)
+    check(out, want, slack)
+    assert not out[0].any()
+    before = randn(g, 100, 40)
+    after = before.clone()
+    assert psb.embedding_grad(grad, tokens, 100, 2.0, padding=0, out=after, accumulate=True) is after
+    # one more addition in FP32: half a step of the result
+    check(after, before.double() + want, slack + (before.double() + want).abs() * U)
+    untouched = want.abs().sum(1) == 0
+    assert untouched.any() and torch.equal(after[untouched], before[untouched])
+    none = tokens[:0]
+    assert not psb.embedding_grad(grad[:0], none, 100).any()
+    psb.embedding_grad(grad[:0], none, 100, out=after, accumulate=True)
+    assert torch.equal(after[untouched], before[untouched])
+    # NaN and inf at empty places reach nothing; at a token they reach its row alone.
+    tokens[5], tokens[6] = -1, 55
+    grad[5], grad[6] = math.nan, math.inf
+    out = psb.embedding_grad(grad, tokens, 100)
+    assert out[55].isinf().all() and out.isfinite().all(1).sum() == 99
+
+
+# ------------------------------------------------------------------------------------ router
+
+def route64(logits, k, normalize):
+    x = logits.double()
+    t, experts = x.shape
+    index = torch.arange(experts, device="cuda")
+    left, chosen = x.clone(), []
+    for _ in range(k):
+        best = left.amax(1)
+        at = torch.where((left == best[:, None]) & (left > -math.inf), index, experts).amin(1)
+        left = left.masked_fill(index == at[:, None], -math.inf)
+        chosen.append(torch.where(at < experts, at, -1))
+    chosen = torch.stack(chosen, 1)
+    on = x > -math.inf
+    if normalize:
+        on &= (index[None, None] == chosen[:, :, None]).any(1)
+    top = torch.where(on, x, -1e300).amax(1, keepdim=True)
+    e = torch.where(on, torch.exp(torch.where(on, x, top) - top), 0.0)
+    p = e / e.sum(1, keepdim=True).clamp_min(1e-300)
+    return p, torch.where(chosen >= 0, p.gather(1, chosen.clamp_min(0)), 0.0), chosen
+
+
+def softmax_slack(logits):
+    """Relative error of a share: x - max rounds by u * |x - max| <= u * spread (in the share's own exponent and, weighted, in
+    the sum), expf is off by 2 steps (4u) in both, the sum of E terms by E * u, the division by u."""
+    x = logits.double()
+    finite = torch.where(x > -math.inf, x, math.nan)
+    spread = (finite.nan_to_num(-1e300).amax(1) - finite.nan_to_num(1e300).amin(1)).clamp_min(0)
+    return (2 * spread + 8 + x.shape[1] + 2)[:, None] * U
+
+
+EXPERTS = [(1, 1), (2, 1), (3, 3), (8, 2), (31, 4), (32, 32), (33, 5), (64, 6), (100, 32), (256, 8), (257, 9), (512, 10), (1024, 32)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("experts,k", EXPERTS)
+def test_route_and_its_gradient(dtype, normalize, experts, k):
+    g = gen(experts)
+    for tokens in (1, 7, 130):
+        logits = randn(g, tokens, experts, dtype=dtype)
+        if tokens == 130:
+            logits[3:9] = -math.inf                                        # no expert at all
+            logits[20:60, ::2] = -math.inf                                 # half of them off
+            logits[60:80] = (logits[60:80].float() * 2).round().to(dtype)  # many ties
+            logits[80:90] = 0.0
+            logits[85:90, 1::2] = -0.0                                     # equal to +0
+            logits[90:95] *= 20
+            logits[95] = torch.finfo(dtype).min                            # the lowest value is a score like any other
+            logits[96, : experts // 2] = torch.finfo(dtype).min
+        p, want, chosen64 = route64(logits, k, normalize)
+        weights, chosen = psb.route(logits, k, normalize)
+        assert torch.equal(chosen.long(), chosen64)
+        slack = softmax_slack(torch.where(logits == torch.finfo(dtype).min, -math.inf, logits))
+        # shares below the smallest normal number lose bits, expf's included
+        check(weights, want, want * slack + 2.0 ** -126)
+        view = strided(logits, 3, 1)
+        again = psb.route(view, k, normalize)
+        assert torch.equal(again[0], weights) and torch.equal(again[1], chosen)
+
+        grad = randn(g, tokens, k)
+        dense = torch.zeros(tokens, experts + 1, dtype=torch.float64, device="cuda")
+        dense.scatter_(1, torch.where(chosen64 >= 0, chosen64, experts), grad.double())
+        dense, on = dense[:, :-1], chosen64 >= 0
+        inner = (grad.double() * weights.double() * on).sum(1, keepdim=True)
+        size = (grad.double() * weights.double() * on).abs().sum(1, keepdim=True)
+        grad_slack = p * (dense.abs() + size) * (slack + (k + 4) * U) + 2.0 ** -126 * (dense.abs() + size + 1)
+        if normalize:  # p is the weights as they were stored
+            p = torch.zeros(tokens, experts + 1, dtype=torch.float64, device="cuda")
+            p = p.scatter_(1, torch.where(on, chosen64, experts), weights.double())[:, :-1]
+        want = p * (dense - inner)
+        got = psb.route_grad(grad, logits, weights, chosen, normalize)
+        check(got, want, grad_slack)
+        out = strided(torch.full_like(logits, 5.0), 1)
+        psb.route_grad(grad, view, weights, chosen, normalize, out=out)
+        assert torch.equal(out, got)
+
+
+def test_route_with_nan_and_inf():
+    logits = randn(gen(1), 5, 40)
+    logits[0, 7] = math.nan
+    logits[1, 3] = math.inf
+    logits[2] = math.nan
+    logits[3, :38] = -math.inf
+    for normalize in (True, False):
+        weights, chosen = psb.route(logits, 4, normalize)
+        assert 7 not in chosen[0].tolist() and weights[0].isnan().all()
+        assert chosen[1, 0] == 3 and weights[1, 0].isnan()
+        assert chosen[2].tolist() == [-1] * 4
+        assert sorted(chosen[3, :2].tolist()) == [38, 39] and chosen[3, 2:].tolist() == [-1, -1]
+        assert weights[3, 2:].tolist() == [0, 0] and abs(weights[3].sum().item() - 1) < 1e-6
+        assert weights[4].isfinite().all()
+        grad = torch.ones(5, 4, device="cuda")
+        grad[3, 2:] = math.nan  # beside a choice of -1: not used
+        got = psb.route_grad(grad, logits, weights, chosen, normalize)
+        assert got[3:].isfinite().all() and got[0].isnan().any()
+
+
+def test_route_gradient_against_differences():
+    logits = randn(gen(2), 6, 12)
+    grad = randn(gen(3), 6, 3).double()
+    for normalize in (True, False):
+        weights, chosen = psb.route(logits, 3, normalize)
+        got = psb.route_grad(grad.float(), logits, weights, chosen, normalize).double()
+        h = 2.0 ** -10
+        for e in range(12):
+            up, down = logits.double(), logits.double()
+            up[:, e] += h
+            down[:, e] -= h
+
+            def value(x):  # the choice held fixed, as the gradient holds it
+                p = torch.softmax(x, 1).gather(1, chosen.long())
+                return ((p / p.sum(1, keepdim=True) if normalize else p) * grad.float().double()).sum(1)
+            # the difference quotient is off by h^2 / 6 of a third derivative (below 10 * |grad|), the kernel by FP32
+            assert ((value(up) - value(down)) / (2 * h) - got[:, e]).abs().max() < 10 * grad.abs().max() * (h * h + 100 * U)
+
+
+# ------------------------------------------------------------------------------------ dispatch and combine
+
+def order64(chosen, experts, align):
+    flat = chosen.reshape(-1).tolist()
+    slots = [[] for _ in range(experts)]
+    for s, e in enumerate(flat):
+        if 0 <= e < experts:
+            slots[e].append(s)
+    position, offsets = [-1] * len(flat), [0]
+    for e in range(experts):
+        for i, s in enumerate(slots[e]):
+            position[s] = offsets[-1] + i
+        offsets.append(offsets[-1] + -(-len(slots[e]) // align) * align)
+    return position, offsets, [len(s) for s in slots]
+
+
+def choices(g, tokens, k, experts, kind, index):
+    if kind == "one":
+        c = torch.full((tokens, k), experts - 1, device="cuda")
+    elif kind == "none":
+        c = torch.full((tokens, k), -1, device="cuda")
+    elif kind == "far":
+        c = torch.randint(0, 2 * experts, (tokens, k), generator=g, device="cuda") - experts // 2
+    else:
+        c = torch.randint(0, experts, (tokens, k), generator=g, device="cuda")  # an expert may come twice
+    return c.to(index)
+
+
+LAYERS = [(1, 1, 1, 1, "any"), (1, 8, 64, 16, "any"), (5, 2, 3, 4, "far"), (33, 6, 64, 1, "any"), (200, 32, 40, 8, "one"),
+          (129, 3, 1024, 1, "far"), (77, 2, 5, 7, "none"), (700, 4, 16, 128, "any"), (3000, 3, 13, 1, "far"), (9000, 8, 384, 16, "any"),
+          (2048, 1, 8, 1, "one"), (341, 6, 9, 2, "any"), (342, 6, 9, 2, "any")]
+
+
+@pytest.mark.parametrize("tokens,k,experts,align,kind", LAYERS)
+@pytest.mark.parametrize("dtype,width", [(F32, 1), (F32, 20), (BF16, 64), (F16, 33), (BF16, 2056), (F16, 6)])
+def test_dispatch_and_combine(tokens, k, experts, align, kind, dtype, width):
+    if tokens * k * width > 2**26:
+        width = 16
+    g = gen(tokens + width)
+    index = torch.int64 if tokens % 2 else torch.int32
+    chosen = choices(g, tokens, k, experts, kind, index)
+    x = randn(g, tokens, width, dtype=dtype)
+    position, offsets, counts = order64(chosen, experts, align)
+    at = torch.tensor(position, device="cuda").view(tokens, k)
+    token, choice = (at >= 0).nonzero(as_tuple=True)
+    slot = at[token, choice]
+    end = offsets[-1]
+    room = psb.dispatch_rows(tokens * k, experts, align)
+    assert end <= room
+
+    want = torch.zeros(room, width, dtype=dtype, device="cuda")
+    want[slot] = x[token]
+    rows, plan = psb.dispatch(x, chosen, experts, align)
+    assert plan.position.tolist() == at.tolist() and plan.offsets.tolist() == offsets and plan.counts.tolist() == counts
+    assert torch.equal(rows, want)
+    out = strided(torch.full((room + 3, width), 9.0, device="cuda", dtype=dtype), 5, 1)
+    psb.dispatch(strided(x, 2), chosen, experts, align, out=out)
+    assert torch.equal(out[:end], want[:end]) and (out[end:] == 9).all()  # the rows behind the last expert stay
+
+    # back, with weights and something added; rows that no token has hold NaN
+    y = randn(g, room, width, dtype=dtype)
+    used = torch.zeros(room, dtype=torch.bool, device="cuda").index_fill_(0, slot, True)
+    y[~used] = math.nan
+    weights = torch.rand(tokens, k, generator=g, device="cuda")
+    weights[at < 0] = math.nan
+    add = randn(g, tokens, width, dtype=dtype)
+    for w, a in ((weights, None), (None, None), (weights, add), (None, add)):
+        sum64 = torch.zeros(tokens, width, dtype=torch.float64, device="cuda")
+        size = sum64.clone()
+        term = y[slot].double() * (1.0 if w is None else w[token, choice].double()[:, None])
+        sum64.index_add_(0, token, term)
+        size.index_add_(0, token, term.abs())
+        if a is not None:
+            sum64, size = sum64 + a.double(), size + a.double().abs()
+        check(psb.combine(y, plan, w, a), sum64, size * (k + 2) * U)
+        dst = strided(torch.zeros(tokens, width, device="cuda", dtype=dtype) if a is None else a, 3, 1)
+        psb.combine(strided(y, 1), plan, w, None if a is None else dst, out=dst)  # add may be out itself
+        check(dst, sum64, size * (k + 2) * U)
+    if kind != "none":
+        assert torch.equal(psb.dispatch_grad(y, plan), psb.combine(y, plan))
+
+    # gradients of combine
+    grad = randn(g, tokens, width, dtype=dtype)
+    grad_y, grad_w = psb.combine_grad(grad, y, plan, weights)
+    want_y = torch.zeros(room, width, dtype=torch.float64, device="cuda")
+    want_y[slot] = weights[token, choice].double()[:, None] * grad[token].double()
+    check(grad_y, want_y, want_y.abs() * U)
+    want_w = torch.zeros(tokens, k, dtype=torch.float64, device="cuda")
+    term = grad[token].double() * y[slot].double()
+    want_w[token, choice] = term.sum(1)
+    size = torch.zeros_like(want_w)
+    size[token, choice] = term.abs().sum(1)
+    check(grad_w, want_w, size * (width / 32 + 24) * U)  # a lane adds at most width / 32 + 8 products, then at most 13 sums
+    out = strided(torch.full((room, width), 9.0, device="cuda", dtype=dtype), 1, 1)
+    again = psb.combine_grad(strided(grad, 1), strided(y, 2), plan, weights, out=out)
+    assert again[0] is out and (out[end:] == 9).all()
+    check(out[:end], want_y[:end], want_y[:end].abs() * U)
+    check(again[1], want_w, size * (width / 32 + 24) * U)
+
+
+def test_no_tokens():
+    x = torch.empty(0, 16, device="cuda", dtype=BF16)
+    rows, plan = psb.dispatch(x, torch.empty(0, 4, dtype=torch.int32, device="cuda"), 8, 128)
+    assert rows.shape == (0, 16) and plan.offsets.tolist() == [0] * 9 and plan.counts.tolist() == [0] * 8
+    assert psb.combine(rows, plan).shape == (0, 16)
+    y = torch.full((5, 16), 2.0, device="cuda", dtype=BF16)
+    grad_y, grad_w = psb.combine_grad(x, y, plan, torch.empty(0, 4, device="cuda"))
+    assert not grad_y.any() and grad_w.shape == (0, 4)
+    weights, chosen = psb.route(torch.empty(0, 8, device="cuda"), 2)
+    assert weights.shape == chosen.shape == (0, 2)
+    assert psb.route_grad(weights, torch.empty(0, 8, device="cuda"), weights, chosen).shape == (0, 8)
+
+
+def test_a_plan_that_points_outside_is_not_followed():
+    """Positions and bounds from anywhere: nothing outside the given tensors is read or written."""
+    far = 2**31 - 1
+    position = torch.tensor([[0, far], [-5, 1], [3, 4]], dtype=torch.int32, device="cuda")
+    plan = psb.DispatchPlan(position, torch.tensor([-7, far, -1], dtype=torch.int32, device="cuda"),
+                            torch.tensor([far, -far], dtype=torch.int32, device="cuda"))
+    y = torch.ones(4, 8, device="cuda")
+    w = torch.ones(3, 2, device="cuda")
+    assert psb.combine(y, plan, w)[:, 0].tolist() == [1, 1, 1]
+    grad_y, grad_w = psb.combine_grad(torch.ones(3, 8, device="cuda"), y, plan, w, out=torch.full_like(y, 9.0))
+    assert grad_w.tolist() == [[8, 0], [0, 8], [8, 0]]
+
+
+def test_dispatch_offsets_pass_32_bits():
+    tokens, k, width = 70_000, 8, 4096  # 2.3e9 elements in expert order
+    x = torch.empty(tokens, width, device="cuda", dtype=BF16)
+    x[:] = (torch.arange(tokens, device="cuda") % 251)[:, None].to(BF16)
+    chosen = torch.arange(k, dtype=torch.int32, device="cuda").repeat(tokens, 1)
+    rows, plan = psb.dispatch(x, chosen, k)
+    assert plan.counts.tolist() == [tokens] * k
+    for e in range(k):
+        assert torch.equal(rows[e * tokens: (e + 1) * tokens: 997], x[::997])
+    assert torch.equal(rows[-1], x[-1])
+    w = torch.full((tokens, k), 0.125, device="cuda")
+    assert torch.equal(psb.combine(rows, plan, w), x)
+    del x
+    grad = torch.ones(tokens, width, device="cuda", dtype=BF16)
+    grad_y, grad_w = psb.combine_grad(grad, rows, plan, w, out=rows)  # each element is read before it is written
+    assert (grad_w[-1] == (tokens - 1) % 251 * width).all() and (grad_y[-1] == 0.125).all() and (grad_y[::1001] == 0.125).all()
+
+
+# ------------------------------------------------------------------------------------ as they are used
+
+def layer(x, logits, experts_w, k, align, ops=torch.ops.powersparse):
+    weights, chosen = ops.route(logits, k, True)
+    rows, position, offsets, counts = ops.dispatch(x, chosen, experts_w.shape[0], align)
+    begin = offsets.tolist()
+    y = torch.cat([torch.tanh(rows[a:b] @ w) for a, b, w in zip(begin, begin[1:], experts_w)] + [rows[begin[-1]:]])
+    return ops.combine(y, position, offsets, counts, weights, x)
+
+
+@pytest.mark.parametrize("align", [1, 4])
+def test_a_model_of_them_and_its_gradients(align):
+    """tokens -> embedding -> router -> dispatch -> experts -> combine with the residual, and back, against autograd in
+    64 bits.  All values are of the order of one and fewer than 500 FP32 roundings lie on any path: 1e-4."""
+    g = gen(11)
+    vocab, width, experts, k = 50, 24, 6, 2
+    tokens = torch.randint(-1, vocab, (4, 20), generator=g, device="cuda")
+    leaves = [randn(g, vocab, width), randn(g, width, experts) * 0.3, randn(g, experts, width, width) * 0.2]
+    ours = [t.clone().requires_grad_() for t in leaves]
+    h = torch.ops.powersparse.embedding(ours[0], tokens, 1.5, 3).view(-1, width)
+    out = layer(h, h @ ours[1], ours[2], k, align)
+    (out * 0.5).sum().backward()  # an expanded gradient
+
+    ref = [t.double().requires_grad_() for t in leaves]
+    flat = tokens.reshape(-1)
+    h = ref[0][flat.clamp_min(0)] * 1.5 * (flat >= 0)[:, None]
+    h = torch.where((flat == 3)[:, None], h.detach(), h)  # token 3 is padding: no gradient through it
+    logits = h @ ref[1]
+    value, chosen = logits.topk(k, 1)
+    weights = torch.softmax(value, 1)
+    every = torch.tanh(torch.einsum("td,edf->tef", h, ref[2]))
+    want = h + (every.gather(1, chosen[:, :, None].expand(-1, -1, width)) * weights[:, :, None]).sum(1)
+    (want * 0.5).sum().backward()
+    # logits that tie (the rows of padding are all zero) choose the same experts in both, up to order; compare all
+    live = (flat >= 0)
+    assert (out.double() - want)[live].abs().max() < 1e-4
+    for a, b in zip(ours, ref):
+        assert (a.grad.double() - b.grad).abs().max() < 1e-4 * max(1.0, b.grad.abs().max().item())
+    assert not ours[0].grad[3].any()
+
+
+def test_gradients_against_differences():
+    """The registered ops' gradients against central differences of the ops themselves (all linear but route, whose own
+    test is above): the difference of a linear map is its gradient up to rounding."""
+    g = gen(4)
+    ops = torch.ops.powersparse
+    chosen = torch.tensor([[0, 2], [1, 1], [-1, 0], [2, 5]], device="cuda")
+    x, w, add = randn(g, 4, 6).requires_grad_(), randn(g, 4, 2).requires_grad_(), randn(g, 4, 6).requires_grad_()
+    probe = randn(g, 4, 6)
+
+    def f(x, w, add):
+        rows, position, offsets, counts = ops.dispatch(x, chosen, 3, 2)
+        return (ops.combine(rows * rows, position, offsets, counts, w, add) * probe).sum()
+    f(x, w, add).backward()
+    for t in (x, w, add):
+        d = randn(g, *t.shape)
+        h = 2.0 ** -6
+        args = [[u.detach() + (s * h * d if u is t else 0) for u in (x, w, add)] for s in (1, -1)]
+        quotient = (f(*args[0]) - f(*args[1])).item() / (2 * h)
+        # f is a polynomial of degree two in each argument, so the quotient is exact; its values round by some u * |f| / h
+        assert abs(quotient - (t.grad * d).sum().item()) < 64 * U / h * 100
+
+
+def test_opcheck():
+    g = gen(6)
+    ops = torch.ops.powersparse
+    which = ("test_schema", "test_faketensor", "test_autograd_registration")
+    table, tokens = randn(g, 20, 8).requires_grad_(), torch.randint(0, 20, (7,), generator=g, device="cuda")
+    torch.library.opcheck(ops.embedding.default, (table, tokens, 2.0, 4), test_utils=which)
+    torch.library.opcheck(ops.embedding_grad.default, (randn(g, 7, 8), tokens, 20), test_utils=which)
+    logits = randn(g, 7, 10).requires_grad_()
+    torch.library.opcheck(ops.route.default, (logits, 3, False), test_utils=which)
+    x, chosen = randn(g, 7, 8).requires_grad_(), torch.randint(0, 5, (7, 3), generator=g, device="cuda")
+    torch.library.opcheck(ops.dispatch.default, (x, chosen, 5, 4), test_utils=which)
+    rows, plan = psb.dispatch(x.detach(), chosen, 5, 4)
+    weights = torch.rand(7, 3, device="cuda").requires_grad_()
+    torch.library.opcheck(ops.combine.default, (rows.requires_grad_(), *plan, weights, x), test_utils=which)
+
+
+def run_all(s):
+    """Every operator once, on tensors of the dictionary `s`."""
+    out = [psb.embedding(s["table"], s["tokens"], 2.0)]
+    out.append(psb.embedding_grad(out[0], s["tokens"], len(s["table"]), 0.5, dtype=F32))
+    weights, chosen = psb.route(s["logits"], 4)
+    rows, plan = psb.dispatch(out[0], chosen, s["logits"].shape[1], 8)
+    y = psb.combine(rows, plan, weights, out[0])
+    grads = psb.combine_grad(y, rows, plan, weights)
+    out += [weights, chosen, rows, *plan, y, *grads, psb.dispatch_grad(grads[0], plan),
+            psb.route_grad(grads[1], s["logits"], weights, chosen)]
+    return out
+
+
+def inputs(seed, n=600):
+    g = gen(seed)
+    return dict(table=randn(g, 300, 72, dtype=BF16), tokens=torch.randint(-1, 300, (n,), generator=g, device="cuda"),
+                logits=randn(g, n, 48, dtype=BF16))
+
+
+def test_replayed_graphs_streams_and_two_at_once():
+    """Captured and replayed with new inputs, on a side stream, and two graphs whose replays overlap: the same bits as
+    eager calls."""
+    sets = [inputs(s) for s in (1, 2, 3, 4)]
+    want = [run_all(s) for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run_all(sets[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+
+    held, graphs, outs = [dict(inputs(9)), dict(inputs(10))], [], []
+    for h in held:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run_all(h))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rounds in ((0, 1), (2, 3), (3, 0)):
+        for h, i in zip(held, rounds):
+            for key in h:
+                h[key].copy_(sets[i][key])
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for graph, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for out, i in zip(outs, rounds):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+def test_explicit_stream_owns_what_the_call_allocates():
+    s = inputs(7)
+    want = run_all(s)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    a = psb.embedding(s["table"], s["tokens"], 2.0, stream=side)
+    b = psb.embedding_grad(a, s["tokens"], 300, 0.5, dtype=F32, stream=side.cuda_stream)
+    weights, chosen = psb.route(s["logits"], 4, stream=side)
+    rows, plan = psb.dispatch(a, chosen, 48, 8, stream=side)
+    y = psb.combine(rows, plan, weights, a, stream=side)
+    side.synchronize()
+    for got, ref in ((a, want[0]), (b, want[1]), (weights, want[2]), (chosen, want[3]), (rows, want[4]), (y, want[8])):
+        assert torch.equal(got, ref)
+
+
+def test_refusals():
+    g = gen(0)
+    x, i = randn(g, 6, 8), torch.zeros(6, 2, dtype=torch.int32, device="cuda")
+    _, plan = psb.dispatch(x, i, 4)
+    y, w = randn(g, 12, 8), torch.ones(6, 2, device="cuda")
+    t = i[:, 0].contiguous()
+    for call in (lambda: psb.embedding(x.double(), t), lambda: psb.embedding(x.t(), t), lambda: psb.embedding(x, t.float()),
+                 lambda: psb.embedding(x, i[:, 0]), lambda: psb.embedding(x, t.cpu()), lambda: psb.embedding(x[0], t),
+                 lambda: psb.embedding(x[:0], t), lambda: psb.embedding(x, t, out=x[:5]), lambda: psb.embedding(x, t, out=x.half()),
+                 lambda: psb.embedding(x[:1].expand(6, 8), t), lambda: psb.embedding(x[:, :0], t),
+                 lambda: psb.embedding_grad(x[:5], t, 4), lambda: psb.embedding_grad(x, t, 0),
+                 lambda: psb.embedding_grad(x, t, 4, dtype=BF16), lambda: psb.embedding_grad(x.half(), t, 4, dtype=BF16),
+                 lambda: psb.embedding_grad(x, t, 4, accumulate=True), lambda: psb.embedding_grad(x, t, 4, padding=4),
+                 lambda: psb.embedding_grad(x, t, 4, out=x), lambda: psb.embedding_grad(x, t, 2**31),
+                 lambda: psb.route(x, 0), lambda: psb.route(x, 9), lambda: psb.route(torch.zeros(2, 1025, device="cuda"), 2),
+                 lambda: psb.route(torch.zeros(2, 64, device="cuda"), 33), lambda: psb.route_grad(w, x, w, i.long()),
+                 lambda: psb.route_grad(w[:5], x, w, i), lambda: psb.route_grad(w, x, w.half(), i),
+                 lambda: psb.dispatch(x, i[:5], 4), lambda: psb.dispatch(x, t, 4), lambda: psb.dispatch(x, i, 0),
+                 lambda: psb.dispatch(x, i, 4, align=0), lambda: psb.dispatch(x, i, 4, out=y[:11]),
+                 lambda: psb.dispatch(x, i, 4, out=y[:, :7]), lambda: psb.dispatch(x, i.t().contiguous().t(), 4),
+                 lambda: psb.dispatch(x, torch.zeros(6, 33, dtype=torch.int32, device="cuda"), 4),
+                 lambda: psb.combine(y, plan, w.half()), lambda: psb.combine(y, plan, w[:5]), lambda: psb.combine(y, plan, add=x[:5]),
+                 lambda: psb.combine(y, plan, add=x.half()), lambda: psb.combine(y, plan._replace(position=i.long())),
+                 lambda: psb.combine(y, plan, out=x[:, :4]), lambda: psb.combine_grad(x[:5], y, plan, w),
+                 lambda: psb.combine_grad(x, y, plan, w, out=y[:11]), lambda: psb.combine_grad(x.half(), y, plan, w),
+                 lambda: psb.combine_grad(x, y, plan._replace(offsets=plan.counts), w)):
+        with pytest.raises(ValueError):
+            call()
