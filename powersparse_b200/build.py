@@ -6,6 +6,7 @@
 Outputs (git-ignored, shipped with the tree):
   powersparse_b200/lib/libpowersparse_b200.so  C ABI + CUDA kernels (include/powersparse_b200.h)
   powersparse_b200/lib/libpowersparse_b200_checked.so   the same with bounds-checked kernels
+  powersparse_b200/lib/_rows.so                native part of powersparse_b200.rows (torch tensors)
   powersparse_b200/lib/libpowersparse.so       the reference's C++ operator API over the C ABI
   powersparse_b200/bin/powersparse_spmm        drop-in benchmark CLI (SpMM)
   powersparse_b200/bin/powersparse_sddmm       drop-in benchmark CLI (SDDMM)
@@ -17,6 +18,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -38,6 +40,7 @@ CUDA_LIB = os.path.join(LIB, "libpowersparse_b200.so")
 # its kernels.  Load it with PSB_LIBRARY=<path> (powersparse_b200.load_library).
 CHECKED_LIB = os.path.join(LIB, "libpowersparse_b200_checked.so")
 CXX_LIB = os.path.join(LIB, "libpowersparse.so")
+ROWS_MODULE = os.path.join(LIB, "_rows.so")
 
 
 def _run(cmd: list[str]) -> None:
@@ -94,9 +97,26 @@ def build_cxx(force: bool = False) -> None:
         _run([HOSTCXX, "-std=c++17", "-O3", "-pthread", "-o", target, *convert])
 
 
+def build_rows_module(force: bool = False) -> str:
+    """The Python module behind powersparse_b200.rows, against the installed torch."""
+    src = os.path.join(CSRC, "python", "rows_module.cpp")
+    os.makedirs(LIB, exist_ok=True)
+    if force or _stale(ROWS_MODULE, [src, os.path.join(INCLUDE, "powersparse_b200.h")]):
+        import torch
+        from torch.utils import cpp_extension
+        includes = cpp_extension.include_paths() + [sysconfig.get_path("include"), INCLUDE,
+                                                    os.path.join(os.path.dirname(CUDA_LIBDIR), "include")]
+        libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+        _run([HOSTCXX, "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+              *("-I" + i for i in includes), "-o", ROWS_MODULE, src, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu",
+              "-lc10_cuda", "-lc10"])
+    return ROWS_MODULE
+
+
 def build_all(force: bool = False) -> None:
     build_cuda(force)
     build_cxx(force)
+    build_rows_module(force)
 
 
 if __name__ == "__main__":
