@@ -162,21 +162,20 @@ __global__ void __launch_bounds__(kSortThreads) expert_order(const void* __restr
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
-  const SortShared sh(smem, experts);
-  const Strip strip = warp_strip(n, rank, blocks);
-  auto digit = [&](long long i) {
+  auto expert = [&](long long i) {
     const long long e = index_at(chosen, wide, i);
     return e >= 0 && e < experts ? int(e) : -1;
   };
   auto widen = [&](uint32_t count) { return (count + uint32_t(align) - 1) / uint32_t(align) * uint32_t(align); };
-  digit_positions(sh, experts, strip, digit, widen, [&](int e, uint32_t begin, uint32_t count) {
-    if (rank != 0) return;
-    offsets[e] = int(begin);
-    counts[e] = int(count);
-    if (e == experts - 1) offsets[experts] = int(begin + widen(count));
-  });
-  place_digits(strip, sh.rows + (threadIdx.x >> 5) * experts, digit,
-               [&](long long i, int d, uint32_t p) { position[i] = d < 0 ? -1 : int(p); });
+  sort_pass<int>(
+      SortShared(smem, experts), experts, 0, warp_strip(n, rank, blocks), expert, [](int e) { return e; }, widen,
+      [&](int e, uint32_t begin, uint32_t count) {
+        if (rank != 0) return;
+        offsets[e] = int(begin);
+        counts[e] = int(count);
+        if (e == experts - 1) offsets[experts] = int(begin + widen(count));
+      },
+      [&](long long i, int e, uint32_t p) { position[i] = e < 0 ? -1 : int(p); });
 }
 
 // ---- rows -----------------------------------------------------------------------
@@ -245,28 +244,24 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsign
   }
 }
 
-template <typename T, int N, bool kWeighted>
+template <typename T, int N, int W, bool kWeighted>
 __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict__ y, long long y_stride, long long rows,
                                                             const int* __restrict__ position, const float* __restrict__ weights,
                                                             const T* add, long long add_stride, int tokens, int top_k, int width,
                                                             T* out, long long out_stride, int lanes_log2) {
   constexpr int kSlots = 4;  // rows in flight
-  const int lanes = 1 << lanes_log2;
+  const int lanes = 1 << lanes_log2, step = lanes * W;
   const long long t = blockIdx.x * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   if (t >= tokens) return;
-  for (int c = (threadIdx.x & (lanes - 1)) * N; c < width; c += lanes * N) {
+  for (int c = (threadIdx.x & (lanes - 1)) * W; c < width; c += lanes * N) {
     float acc[N];
-    if (add) {
-      Pack<T, N> a;
-      a.load_rw(add + t * add_stride + c);
+    Pack<T, N, W> o;
+    o.zero();
+    if (add) o.load_rw(add + t * add_stride, c, step, width);
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = a.get(e);
-    } else {
-#pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = 0.f;
-    }
+    for (int e = 0; e < N; ++e) acc[e] = o.get(e);
     for (int j0 = 0; j0 < top_k; j0 += kSlots) {
-      Pack<T, N> v[kSlots];
+      Pack<T, N, W> v[kSlots];
       float w[kSlots];
       bool on[kSlots];
 #pragma unroll
@@ -274,7 +269,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict_
         const int p = j0 + s < top_k ? position[t * top_k + j0 + s] : -1;
         on[s] = p >= 0 && p < rows;
         if (on[s]) {
-          v[s].load(y + p * y_stride + c);
+          v[s].load(y + p * y_stride, c, step, width);
           w[s] = kWeighted ? weights[t * top_k + j0 + s] : 1.f;
         }
       }
@@ -285,27 +280,25 @@ __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict_
           for (int e = 0; e < N; ++e) acc[e] += w[s] * v[s].get(e);
         }
     }
-    Pack<T, N> o;
 #pragma unroll
     for (int e = 0; e < N; ++e) o.set(e, acc[e]);
-    o.store(out + t * out_stride + c);
+    o.store(out + t * out_stride, c, step, width);
   }
 }
 
-template <typename T, int N>
-__global__ void __launch_bounds__(kRowThreads) combine_grad_rows(const T* __restrict__ grad, long long grad_stride,
-                                                                 const T* __restrict__ y, long long y_stride,
-                                                                 const int* __restrict__ position, Blanks blanks,
-                                                                 const float* __restrict__ weights, int tokens, int top_k,
-                                                                 int width, T* __restrict__ grad_y, long long grad_y_stride,
+template <typename T, int N, int W>
+__global__ void __launch_bounds__(kRowThreads) combine_grad_rows(const T* __restrict__ grad, long long grad_stride, const T* y,
+                                                                 long long y_stride, const int* __restrict__ position,
+                                                                 Blanks blanks, const float* __restrict__ weights, int tokens,
+                                                                 int top_k, int width, T* grad_y, long long grad_y_stride,
                                                                  float* __restrict__ grad_weights, int lanes_log2) {
   constexpr int kSlots = 8;  // rows in flight, and dot products held
-  constexpr int kBytes = N * int(sizeof(T));
   if (int(blockIdx.x) < blanks.blocks())
-    return zero_blanks<kBytes>(blanks, width / N, reinterpret_cast<unsigned char*>(grad_y), grad_y_stride * (long long)sizeof(T));
+    return zero_blanks<W * int(sizeof(T))>(blanks, width / W, reinterpret_cast<unsigned char*>(grad_y),
+                                           grad_y_stride * (long long)sizeof(T));
   const long long rows = blanks.rows;
   __shared__ float parts[kRowThreads / 32][kSlots];
-  const int lanes = 1 << lanes_log2;  // 32 at least
+  const int lanes = 1 << lanes_log2, step = lanes * W;  // 32 lanes at least
   const long long t = (blockIdx.x - blanks.blocks()) * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   const bool live = t < tokens;  // the whole warp; the others take part in the block's barriers
   for (int j0 = 0; j0 < top_k; j0 += kSlots) {
@@ -320,22 +313,25 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_rows(const T* __rest
       dot[s] = 0.f;
     }
     if (live) {
-      for (int c = (threadIdx.x & (lanes - 1)) * N; c < width; c += lanes * N) {
-        Pack<T, N> g, v[kSlots];
-        g.load(grad + t * grad_stride + c);
+      for (int c = (threadIdx.x & (lanes - 1)) * W; c < width; c += lanes * N) {
+        Pack<T, N, W> g, v[kSlots];
+        g.zero();
+        g.load(grad + t * grad_stride, c, step, width);
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s)
-          if (p[s] >= 0) v[s].load(y + p[s] * y_stride + c);
+        for (int s = 0; s < kSlots; ++s) {
+          if (N != W) v[s].zero();  // columns behind the row
+          if (p[s] >= 0) v[s].load_rw(y + p[s] * y_stride, c, step, width);
+        }
 #pragma unroll
         for (int s = 0; s < kSlots; ++s) {
           if (p[s] < 0) continue;
-          Pack<T, N> o;
+          Pack<T, N, W> o;
 #pragma unroll
           for (int e = 0; e < N; ++e) {
             dot[s] += g.get(e) * v[s].get(e);
             o.set(e, w[s] * g.get(e));
           }
-          o.store(grad_y + p[s] * grad_y_stride + c);
+          o.store(grad_y + p[s] * grad_y_stride, c, step, width);
         }
       }
     }
@@ -373,11 +369,6 @@ void with_scores(int experts, F&& f) {
   else if (experts <= 256) f(Count<8>());
   else if (experts <= 512) f(Count<16>());
   else f(Count<32>());
-}
-
-// log2 of the threads that share a row of `words` words, `each` of them a thread.
-int row_lanes(int words, int each, int least_log2) {
-  return std::min(8, std::max(least_log2, log2_up(ceil_div(words, each))));
 }
 
 int tail_blocks(bool zero_tail, long long rows) {
@@ -422,8 +413,8 @@ long long dispatch_rows(long long slots, int experts, int align) {
 void dispatch_launch(int dtype, RowsIn x, Indices chosen, int tokens, int top_k, int experts, int align, int width, RowsOut out,
                      long long row_count, bool zero_tail, int* position, int* offsets, int* counts, cudaStream_t stream) {
   const long long n = chosen.count;
-  launch_cluster(expert_order, sort_blocks(n), sort_smem(experts), stream, chosen.ptr, chosen.wide, n, experts, align, position,
-                 offsets, counts);
+  launch_clusters<expert_order>(sort_blocks(n), 1, experts, stream, chosen.ptr, chosen.wide, n, experts, align, position, offsets,
+                                counts);
   const Blanks blanks{offsets, counts, row_count, experts, tail_blocks(zero_tail, row_count), align > 1 ? experts * kPadBlocks : 0};
   if (n == 0 && blanks.tail == 0) return;
   const int size = dtype_size(dtype);
@@ -451,21 +442,19 @@ void combine_launch(int dtype, RowsIn y, long long rows, const int* position, co
   const int size = dtype_size(dtype);
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto per) {
-      constexpr int N = decltype(per)::value;
+    auto fits = [&](int bytes) {
+      return rows_aligned(y.ptr, y.stride, size, bytes) && rows_aligned(out.ptr, out.stride, size, bytes) &&
+             (!add.ptr || rows_aligned(add.ptr, add.stride, size, bytes));
+    };
+    with_shape<T>(width, fits, [&](auto shape) {
+      constexpr int N = decltype(shape)::N, W = decltype(shape)::W;
       const int lanes_log2 = row_lanes(ceil_div(width, N), 2, 0);
       const unsigned blocks = grid_x(ceil_div_ll(tokens, kRowThreads >> lanes_log2));
-      auto kernel = weights ? combine_rows<T, N, true> : combine_rows<T, N, false>;
+      auto kernel = weights ? combine_rows<T, N, W, true> : combine_rows<T, N, W, false>;
       kernel<<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(y.ptr), y.stride, rows, position, weights,
                                                  static_cast<const T*>(add.ptr), add.stride, tokens, top_k, width,
                                                  static_cast<T*>(out.ptr), out.stride, lanes_log2);
-    };
-    constexpr int kWide = 16 / sizeof(T);
-    if (width % kWide == 0 && rows_aligned(y.ptr, y.stride, size, 16) && rows_aligned(out.ptr, out.stride, size, 16) &&
-        (!add.ptr || rows_aligned(add.ptr, add.stride, size, 16)))
-      run(Count<kWide>());
-    else
-      run(Count<1>());
+    });
   });
   PSB_LAUNCH_CHECK();
 }
@@ -477,20 +466,18 @@ void combine_grad_launch(int dtype, RowsIn grad, RowsIn y, long long rows, const
   const int size = dtype_size(dtype);
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    auto run = [&](auto per) {
-      constexpr int N = decltype(per)::value;
+    auto fits = [&](int bytes) {
+      return rows_aligned(grad.ptr, grad.stride, size, bytes) && rows_aligned(y.ptr, y.stride, size, bytes) &&
+             rows_aligned(grad_y.ptr, grad_y.stride, size, bytes);
+    };
+    with_shape<T>(width, fits, [&](auto shape) {
+      constexpr int N = decltype(shape)::N, W = decltype(shape)::W;
       const int lanes_log2 = row_lanes(ceil_div(width, N), 8, 5);
       const unsigned blocks = grid_x(blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2));
-      combine_grad_rows<T, N><<<blocks, kRowThreads, 0, stream>>>(
-          static_cast<const T*>(grad.ptr), grad.stride, static_cast<const T*>(y.ptr), y.stride, position, blanks,
-          weights, tokens, top_k, width, static_cast<T*>(grad_y.ptr), grad_y.stride, grad_weights, lanes_log2);
-    };
-    constexpr int kWide = 16 / sizeof(T);
-    if (width % kWide == 0 && rows_aligned(grad.ptr, grad.stride, size, 16) && rows_aligned(y.ptr, y.stride, size, 16) &&
-        rows_aligned(grad_y.ptr, grad_y.stride, size, 16))
-      run(Count<kWide>());
-    else
-      run(Count<1>());
+      combine_grad_rows<T, N, W><<<blocks, kRowThreads, 0, stream>>>(
+          static_cast<const T*>(grad.ptr), grad.stride, static_cast<const T*>(y.ptr), y.stride, position, blanks, weights, tokens,
+          top_k, width, static_cast<T*>(grad_y.ptr), grad_y.stride, grad_weights, lanes_log2);
+    });
   });
   PSB_LAUNCH_CHECK();
 }

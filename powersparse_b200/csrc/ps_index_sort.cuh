@@ -5,17 +5,21 @@
 // counters a warp, so no atomics), turns the counts into the position of each
 // strip's first element of each digit (a sum over the warps of the block, over the
 // earlier blocks of the cluster through distributed shared memory, and over the
-// smaller digits), and walks the strips again to place every element: 32 elements at
-// a time, in order, ranked among the lanes of equal digit.  Nothing depends on
-// timing, so equal keys keep their order and two runs give the same result.
+// smaller digits), and places every element: 32 elements at a time, in order, ranked
+// among the lanes of equal digit.  Nothing depends on timing, so equal digits keep
+// their order and two runs give the same result.
 //
 // Why one cluster: at the sizes of a batch (10^4 to 10^5 indices) the passes over the
-// data are short and the launches and the counters' round trips through memory between
-// them are what costs.  The hardware's cluster barrier orders the passes (it also
-// makes their global writes visible to the cluster), without a wait on memory.
+// data are short, and launches and counters that go through memory between them are
+// what costs.  The hardware's cluster barrier orders the passes (it also makes their
+// global writes visible to the cluster), without a wait on memory.  A strip of up to
+// kKeep * 32 elements stays in registers between counting and placing, its ranks with
+// it; a longer one is walked twice.
 #pragma once
 
 #include <cooperative_groups.h>
+
+#include <utility>
 
 #include "ps_common.cuh"
 
@@ -23,7 +27,8 @@ namespace psb {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortUnroll = 8;  // loads in flight a lane
+constexpr int kMaxDigits = 1024;  // one thread a digit
+constexpr int kKeep = 8;
 
 struct Strip {
   long long begin, end;
@@ -37,49 +42,16 @@ __device__ __forceinline__ Strip warp_strip(long long n, int rank, int blocks) {
   return {b < n ? b : n, b + len < n ? b + len : n};
 }
 
-// row[d] += elements of the strip with digit d (digit(i) < 0: not counted).
-template <typename Digit>
-__device__ __forceinline__ void count_digits(Strip s, uint32_t* row, Digit&& digit) {
+// row[d] of the lanes' digits d (-1: none) before this chunk of 32, plus the number of
+// lower lanes of the same digit; row[d] is counted up.
+__device__ __forceinline__ uint32_t rank_chunk(uint32_t* row, int d) {
   const int lane = threadIdx.x & 31;
-  for (long long base = s.begin; base < s.end; base += 32 * kSortUnroll) {
-    int d[kSortUnroll];
-#pragma unroll
-    for (int u = 0; u < kSortUnroll; ++u) {
-      const long long i = base + u * 32 + lane;
-      d[u] = i < s.end ? digit(i) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kSortUnroll; ++u) {
-      const unsigned same = __match_any_sync(0xffffffffu, d[u]);
-      if (d[u] >= 0 && lane == __ffs(same) - 1) row[d[u]] += __popc(same);
-      __syncwarp();
-    }
-  }
-}
-
-// place(i, p) for every element of the strip: p = row[digit] counted up in order
-// (p is not meaningful where digit(i) < 0).
-template <typename Digit, typename Place>
-__device__ __forceinline__ void place_digits(Strip s, uint32_t* row, Digit&& digit, Place&& place) {
-  const int lane = threadIdx.x & 31;
-  for (long long base = s.begin; base < s.end; base += 32 * kSortUnroll) {
-    int d[kSortUnroll];
-#pragma unroll
-    for (int u = 0; u < kSortUnroll; ++u) {
-      const long long i = base + u * 32 + lane;
-      d[u] = i < s.end ? digit(i) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kSortUnroll; ++u) {
-      const unsigned same = __match_any_sync(0xffffffffu, d[u]);
-      const uint32_t first = d[u] >= 0 ? row[d[u]] : 0u;
-      __syncwarp();
-      if (d[u] >= 0 && lane == __ffs(same) - 1) row[d[u]] = first + __popc(same);
-      __syncwarp();
-      const long long i = base + u * 32 + lane;
-      if (i < s.end) place(i, d[u], first + __popc(same & ((1u << lane) - 1u)));
-    }
-  }
+  const unsigned same = __match_any_sync(0xffffffffu, d);
+  const uint32_t first = d >= 0 ? row[d] : 0u;
+  __syncwarp();
+  if (d >= 0 && lane == __ffs(same) - 1) row[d] = first + __popc(same);
+  __syncwarp();
+  return first + __popc(same & ((1u << lane) - 1u));
 }
 
 // Exclusive sum over the block's threads; `scratch` holds kSortWarps words.
@@ -94,7 +66,8 @@ __device__ __forceinline__ uint32_t block_sum_before(uint32_t v, uint32_t* scrat
   if (lane == 31) scratch[warp] = inc;
   __syncthreads();
   if (warp == 0) {
-    uint32_t w = lane < kSortWarps ? scratch[lane] : 0u, winc = w;
+    const uint32_t w = lane < kSortWarps ? scratch[lane] : 0u;
+    uint32_t winc = w;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const uint32_t o = __shfl_up_sync(0xffffffffu, winc, d);
@@ -103,75 +76,142 @@ __device__ __forceinline__ uint32_t block_sum_before(uint32_t v, uint32_t* scrat
     if (lane < kSortWarps) scratch[lane] = winc - w;
   }
   __syncthreads();
-  const uint32_t before = scratch[warp] + inc - v;
-  __syncthreads();
-  return before;
+  return scratch[warp] + inc - v;
 }
 
-// Shared memory of a pass: kSortWarps rows of `digits` counters, the block's totals and scratch.
-inline size_t sort_smem(int digits) { return sizeof(uint32_t) * (size_t(kSortWarps) * digits + digits + kSortWarps); }
-
+// Shared memory of a sort: kSortWarps rows of counters (an odd pitch, so that a warp
+// reads a column without bank conflicts), two sets of block totals (one pass writes
+// one while a slower block may still read the other), the digits' bases and scratch.
 struct SortShared {
-  uint32_t* rows;     // [kSortWarps][digits]
-  uint32_t* total;    // [digits]: this block's count of each digit
-  uint32_t* scratch;  // [kSortWarps]
+  uint32_t* rows;
+  uint32_t* total;
+  uint32_t* base;
+  uint32_t* scratch;
+  int pitch;
   __device__ SortShared(uint32_t* smem, int digits)
-      : rows(smem), total(smem + kSortWarps * digits), scratch(total + digits) {}
+      : rows(smem),
+        total(smem + kSortWarps * (digits | 1)),
+        base(total + 2 * digits),
+        scratch(base + digits),
+        pitch(digits | 1) {}
 };
+inline size_t sort_smem(int digits) {
+  return sizeof(uint32_t) * (size_t(kSortWarps) * (digits | 1) + 3 * size_t(digits) + kSortWarps);
+}
 
-// One digit pass up to the counters: afterwards sh.rows[w][d] is the position of the
-// first element with digit d of warp w's strip.  `widen(count)` is the room that the
-// elements of a digit take (at least count); `report(d, begin, count)` is called by
-// one thread a digit in every block.  digits <= kSortThreads.
-template <typename Digit, typename Widen, typename Report>
-__device__ __forceinline__ void digit_positions(SortShared sh, int digits, Strip strip, Digit&& digit, Widen&& widen,
-                                                Report&& report) {
+// One pass: place(i, element, p) for every element of the strip, p its position in the
+// stable order by digit.  load(i) gives the element i, digit_of(element) its digit (-1:
+// the element is not counted, and p means nothing).  widen(count) is the room that the
+// elements of a digit take (at least count); report(d, begin, count) is called by one
+// thread a digit in every block.  Ends with the cluster's barrier.
+template <typename Element, typename Load, typename DigitOf, typename Widen, typename Report, typename Place>
+__device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity, Strip strip, Load&& load, DigitOf&& digit_of,
+                                          Widen&& widen, Report&& report, Place&& place) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
-  for (int i = threadIdx.x; i < kSortWarps * digits; i += kSortThreads) sh.rows[i] = 0;
-  __syncthreads();
-  count_digits(strip, sh.rows + (threadIdx.x >> 5) * digits, digit);
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d < digits) {
-    uint32_t sum = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t c = sh.rows[w * digits + d];
-      sh.rows[w * digits + d] = sum;
-      sum += c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t* row = sh.rows + warp * sh.pitch;
+  for (int d = lane; d < digits; d += 32) row[d] = 0;
+  __syncwarp();
+
+  const bool kept = strip.end - strip.begin <= kKeep * 32;
+  Element e[kKeep];
+  uint32_t r[kKeep];
+  for (long long base = strip.begin; base < strip.end; base += kKeep * 32) {
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u) {
+      const long long i = base + u * 32 + lane;
+      if (i < strip.end) e[u] = load(i);
     }
-    sh.total[d] = sum;
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u)
+      if (base + u * 32 < strip.end) r[u] = rank_chunk(row, base + u * 32 + lane < strip.end ? digit_of(e[u]) : -1);
+  }
+  __syncthreads();
+
+  // Counts to positions within the block: a warp takes every kSortWarps-th digit, a lane
+  // the counter of one warp.
+  for (int d = warp; d < digits; d += kSortWarps) {
+    const uint32_t c = sh.rows[lane * sh.pitch + d];
+    uint32_t inc = c;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, inc, s);
+      if (lane >= s) inc += o;
+    }
+    sh.rows[lane * sh.pitch + d] = inc - c;
+    if (lane == 31) sh.total[parity * digits + d] = inc;
   }
   cluster.sync();
+
+  const int d = threadIdx.x;
   uint32_t count = 0, earlier = 0;
   if (d < digits) {
     for (int b = 0; b < blocks; ++b) {
-      const uint32_t c = cluster.map_shared_rank(sh.total, b)[d];
+      const uint32_t c = cluster.map_shared_rank(sh.total, b)[parity * digits + d];
       if (b < rank) earlier += c;
       count += c;
     }
   }
-  cluster.sync();  // the totals have been read: a later pass may write them, a block may end
   const uint32_t begin = block_sum_before(d < digits ? widen(count) : 0u, sh.scratch);
   if (d < digits) {
     report(d, begin, count);
-    for (int w = 0; w < kSortWarps; ++w) sh.rows[w * digits + d] += begin + earlier;
+    sh.base[d] = begin + earlier;
   }
   __syncthreads();
+
+  if (kept) {
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u) {
+      const long long i = strip.begin + u * 32 + lane;
+      if (i < strip.end) {
+        const int digit = digit_of(e[u]);
+        place(i, e[u], digit < 0 ? 0u : sh.base[digit] + row[digit] + r[u]);
+      }
+    }
+  } else {
+    for (long long base = strip.begin; base < strip.end; base += kKeep * 32) {
+#pragma unroll
+      for (int u = 0; u < kKeep; ++u) {
+        const long long i = base + u * 32 + lane;
+        if (i < strip.end) e[u] = load(i);
+      }
+#pragma unroll
+      for (int u = 0; u < kKeep; ++u) {
+        if (base + u * 32 >= strip.end) break;
+        const long long i = base + u * 32 + lane;
+        const int digit = i < strip.end ? digit_of(e[u]) : -1;
+        const uint32_t p = rank_chunk(row, digit);
+        if (i < strip.end) place(i, e[u], digit < 0 ? 0u : sh.base[digit] + p);
+      }
+    }
+  }
+  // The places are visible to the cluster, and no block ends (or counts again) while
+  // another may read its totals.
+  cluster.sync();
 }
 
-// Blocks of the cluster for n indices: one while a block's warps each have one short
-// strip, more as the strips grow (8 is the largest cluster that every sm_100 GPU takes).
+// Blocks of the cluster for n indices: one while each warp's strip is short, more as
+// the strips grow (8 is the largest cluster that needs no opt-in).
 inline int sort_blocks(long long n) { return n <= 2048 ? 1 : n <= 8192 ? 4 : 8; }
 
-template <typename... Params, typename... Args>
-void launch_cluster(void (*kernel)(Params...), int blocks, size_t smem, cudaStream_t stream, Args&&... args) {
-  PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+// Launches `kernel` with `clusters` clusters of `blocks` blocks of kSortThreads.
+template <auto kernel, typename... Args>
+void launch_clusters(int blocks, long long clusters, int digits, cudaStream_t stream, Args... args) {
+  static std::atomic<unsigned long long> prepared{0};  // devices on which the kernel may take its largest shared memory
+  int device = 0;
+  PSB_CUDA(cudaGetDevice(&device));
+  const unsigned long long bit = device < 64 ? 1ULL << device : 0;
+  if (!(prepared.load(std::memory_order_relaxed) & bit)) {
+    PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sort_smem(kMaxDigits))));
+    prepared.fetch_or(bit, std::memory_order_relaxed);
+  }
+  if (clusters * blocks > 0x7fffffffLL) throw std::invalid_argument("too many rows for one launch");
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(blocks);
+  config.gridDim = dim3(unsigned(clusters * blocks));
   config.blockDim = dim3(kSortThreads);
-  config.dynamicSmemBytes = smem;
+  config.dynamicSmemBytes = sort_smem(digits);
   config.stream = stream;
   cudaLaunchAttribute attr[1] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -179,7 +219,7 @@ void launch_cluster(void (*kernel)(Params...), int blocks, size_t smem, cudaStre
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = 1;
-  PSB_CUDA(cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...));
+  PSB_CUDA(cudaLaunchKernelEx(&config, kernel, args...));
 }
 
 }  // namespace psb

@@ -36,34 +36,52 @@ template <> struct WordOf<4> { using type = uint32_t; };
 template <> struct WordOf<2> { using type = uint16_t; };
 template <int B> using Word = typename WordOf<B>::type;
 
-// N consecutive elements of a row, moved in words of at most 16 bytes.
-template <typename T, int N>
+// What a thread holds of a row: N elements as N / W words of W, the words `step`
+// columns apart (the threads that share the row stand side by side).  Where rows begin
+// at multiples of 16 bytes W = N and a word is 16 bytes of T; where they do not, W is
+// smaller and the thread still has the same bytes in flight.
+template <typename T, int N, int W>
 struct Pack {
-  static constexpr int kWord = N * int(sizeof(T)) < 16 ? N * int(sizeof(T)) : 16;
-  static constexpr int kWords = N * int(sizeof(T)) / kWord;
+  static constexpr int kWordBytes = W * int(sizeof(T));
+  static constexpr int kPart = kWordBytes < 16 ? kWordBytes : 16;
+  static constexpr int kParts = kWordBytes / kPart;
+  using Part = Word<kPart>;
   union {
-    Word<kWord> w[kWords];
+    Part w[N / W][kParts];
     unsigned char bytes[N * sizeof(T)];
   };
-  __device__ __forceinline__ void load(const T* p) {
+  // The words at columns c, c + step, ... of a row, as far as they lie below `width`
+  // (a word lies below it or not as a whole).
+  __device__ __forceinline__ void load(const T* row, int c, int step, int width) {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = __ldg(reinterpret_cast<const Word<kWord>*>(p) + i);
+    for (int i = 0; i < N / W; ++i)
+      if (c + i * step < width)
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) w[i][k] = __ldg(reinterpret_cast<const Part*>(row + c + i * step) + k);
   }
   // For memory that this kernel also writes.
-  __device__ __forceinline__ void load_rw(const T* p) {
+  __device__ __forceinline__ void load_rw(const T* row, int c, int step, int width) {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = *(reinterpret_cast<const Word<kWord>*>(p) + i);
+    for (int i = 0; i < N / W; ++i)
+      if (c + i * step < width)
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) w[i][k] = *(reinterpret_cast<const Part*>(row + c + i * step) + k);
   }
-  __device__ __forceinline__ void store(T* p) const {
+  __device__ __forceinline__ void store(T* row, int c, int step, int width) const {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) reinterpret_cast<Word<kWord>*>(p)[i] = w[i];
+    for (int i = 0; i < N / W; ++i)
+      if (c + i * step < width)
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) reinterpret_cast<Part*>(row + c + i * step)[k] = w[i][k];
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) w[i] = Word<kWord>{};
+    for (int i = 0; i < N / W; ++i)
+#pragma unroll
+      for (int k = 0; k < kParts; ++k) w[i][k] = Part{};
   }
-  __device__ __forceinline__ float get(int i) const { return to_float(reinterpret_cast<const T*>(bytes)[i]); }
-  __device__ __forceinline__ void set(int i, float x) { reinterpret_cast<T*>(bytes)[i] = from_float<T>(x); }
+  __device__ __forceinline__ float get(int e) const { return to_float(reinterpret_cast<const T*>(bytes)[e]); }
+  __device__ __forceinline__ void set(int e, float x) { reinterpret_cast<T*>(bytes)[e] = from_float<T>(x); }
 };
 
 __device__ __forceinline__ long long index_at(const void* p, bool wide, long long i) {
@@ -83,11 +101,33 @@ inline bool rows_aligned(const void* ptr, long long stride, int size, int bytes)
   return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && (stride * size) % bytes == 0;
 }
 
+// Elements a thread holds (N) and elements of a word (W).
+template <int N_, int W_>
+struct Shape {
+  static constexpr int N = N_, W = W_;
+};
+
+// Calls f(Shape) for rows of `width` elements of type T: words of 16 bytes where
+// fits(16) says that every operand's rows allow them, of 4 bytes where fits(4) does,
+// else single elements.  fits need not look at the width.
+template <typename T, typename Fits, typename F>
+void with_shape(int width, Fits&& fits, F&& f) {
+  constexpr int kSize = int(sizeof(T)), kN = 16 / kSize, kHalf = 4 / kSize;
+  if (width % kN == 0 && fits(16)) f(Shape<kN, kN>());
+  else if (kHalf > 1 && width % kHalf == 0 && fits(4)) f(Shape<kN, kHalf>());
+  else f(Shape<kN, 1>());
+}
+
 // log2 of the smallest power of two >= v.
 inline int log2_up(long long v) {
   int b = 0;
   while ((1LL << b) < v) ++b;
   return b;
+}
+
+// log2 of the threads that share a row of `words` words, `each` of them a thread.
+inline int row_lanes(int words, int each, int least_log2) {
+  return std::min(8, std::max(least_log2, log2_up(ceil_div(words, each))));
 }
 
 inline unsigned grid_x(long long blocks) {
