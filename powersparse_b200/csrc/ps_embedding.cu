@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  let_next_start();
   if (int(blockIdx.x) >= blocks) return zeros.run(blockIdx.x - blocks);
   const int digits = 1 << pass_bits;
   const SortShared sh(smem, digits);
@@ -147,7 +148,7 @@ __device__ __forceinline__ void write_sum(O* row, int c, int step, int width, co
 
 template <typename T, typename O, int N, int W>
 __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ grad, long long grad_stride,
-                                                        const Item* __restrict__ items, long long n, uint32_t rows, int width, float scale, bool accumulate,
+                                                        const Item* items, long long n, uint32_t rows, int width, float scale, bool accumulate,
                                                         O* __restrict__ out, long long out_stride, int chunk,
                                                         float* __restrict__ partial) {
   constexpr int kUnroll = 8;
@@ -155,6 +156,8 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
   __shared__ uint32_t key[kMaxChunk + 2], at[kMaxChunk];
   const long long first = blockIdx.x * (long long)chunk;
   const int count = int(min((long long)chunk, n - first));
+  let_next_start();
+  wait_for_previous();
   for (int i = threadIdx.x; i < count + 2; i += kSumThreads) {
     const long long p = first + i - 1;
     const Item item = p >= 0 && p < n ? items[p] : Item{kNone, 0};
@@ -204,13 +207,13 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
 constexpr int kJoinWarps = 8;
 
 template <typename O, int N, int W>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* __restrict__ items, long long n, int width, float scale,
+__global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, long long n, int width, float scale,
                                                              bool accumulate, O* __restrict__ out, long long out_stride, int chunk,
-                                                             const float* __restrict__ partial, const int* __restrict__ joins,
-                                                             const int* __restrict__ join_count) {
+                                                             const float* partial, const int* joins, const int* join_count) {
   __shared__ float sums[kJoinWarps][32 * N];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slabs = ceil_div(width, 32 * N);
+  wait_for_previous();
   const long long work = (long long)*join_count * slabs;
   for (long long item = blockIdx.x; item < work; item += gridDim.x) {
     const long long own = joins[item / slabs];
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* __restr
       if (c < width) {
         Pack<float, N, W> v;
         v.zero();
-        v.load(partial + (j * 2 + (j == own ? 1 : 0)) * width, c, 32 * W, width);
+        v.load_rw(partial + (j * 2 + (j == own ? 1 : 0)) * width, c, 32 * W, width);
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] += v.get(e);
       }
@@ -314,14 +317,12 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
       O* dst = static_cast<O*>(out.ptr);
       const unsigned chunks = grid_x(ceil_div_ll(n, chunk));
       const dim3 sums(chunks, unsigned(ceil_div(width, kSumThreads * N)));
-      sum_runs<T, O, N, W><<<sums, kSumThreads, 0, stream>>>(static_cast<const T*>(grad.ptr), grad.stride, items, n, uint32_t(rows),
-                                                             width, scale, accumulate, dst, out.stride, chunk, partial);
-      PSB_LAUNCH_CHECK();
+      launch_after(sum_runs<T, O, N, W>, sums, kSumThreads, stream, static_cast<const T*>(grad.ptr), grad.stride, items, n,
+                   uint32_t(rows), width, scale, accumulate, dst, out.stride, chunk, partial);
       if (chunks == 1) return;
       const long long work = (long long)(chunks - 1) * ceil_div(width, 32 * N);
-      join_runs<O, N, W><<<unsigned(std::min<long long>(work, 4LL * device_sms())), kJoinWarps * 32, 0, stream>>>(
-          items, n, width, scale, accumulate, dst, out.stride, chunk, partial, joins, join_count);
-      PSB_LAUNCH_CHECK();
+      launch_after(join_runs<O, N, W>, unsigned(std::min<long long>(work, 4LL * device_sms())), kJoinWarps * 32, stream, items, n,
+                   width, scale, accumulate, dst, out.stride, chunk, partial, joins, join_count);
     });
   };
   with_type(grad_dtype, [&](auto t) {

@@ -57,51 +57,107 @@ __device__ __forceinline__ void row_softmax(const float (&x)[V], float& top, flo
   sum = warp_sum(sum);
 }
 
+// The top_k largest of a warp's keys (0: never taken), ranked: take(r, key, index) is
+// called by one lane for every rank r that there is; returns their number.
+//
+// The k-th largest of the 32 lanes' own maxima is a bound that at least k keys reach,
+// and rarely many more do: those are gathered in shared memory and each lane ranks one
+// of them among all.  Where more than 32 reach it (equal scores), the keys are taken
+// one by one instead, as they are for few choices, where that is faster.
+constexpr int kTakeOneByOne = 3;
+
+template <int V, typename Take>
+__device__ __forceinline__ int top_keys(uint32_t (&key)[V], int top_k, uint2* room, Take&& take) {
+  const int lane = threadIdx.x & 31;
+  uint32_t best = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) best = max(best, key[v]);
+  if (top_k > kTakeOneByOne) {
+    uint32_t sorted = best;  // bitonic, largest first
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+      for (int stride = size / 2; stride > 0; stride /= 2) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, sorted, stride);
+        const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
+        sorted = larger ? max(sorted, other) : min(sorted, other);
+      }
+    const uint32_t bound = max(1u, __shfl_sync(0xffffffffu, sorted, top_k - 1));
+    int found = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const unsigned reach = __ballot_sync(0xffffffffu, key[v] >= bound);
+      const int slot = found + __popc(reach & ((1u << lane) - 1u));
+      if (key[v] >= bound && slot < 32) room[slot] = make_uint2(key[v], v * 32 + lane);
+      found += __popc(reach);
+    }
+    if (found <= 32) {
+      __syncwarp();
+      const uint2 mine = lane < found ? room[lane] : make_uint2(0, 0);
+      int rank = 0;  // the slots ascend with the index: of equal keys the lower slot first
+      for (int i = 0; i < found; ++i) {
+        const uint32_t other = room[i].x;
+        rank += other > mine.x || (other == mine.x && i < lane);
+      }
+      if (lane < found && rank < top_k) take(rank, mine.x, int(mine.y));
+      return min(found, top_k);
+    }
+  }
+  for (int j = 0; j < top_k; ++j) {
+    const uint32_t largest = __reduce_max_sync(0xffffffffu, best);
+    if (largest == 0) return j;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v)
+      if (key[v] == largest) at = v * 32 + lane;
+    const int first = __reduce_min_sync(0xffffffffu, at);
+    best = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (first == v * 32 + lane) key[v] = 0;
+      best = max(best, key[v]);
+    }
+    if (at == first) take(j, largest, first);
+  }
+  return top_k;
+}
+
+__device__ __forceinline__ float unordered(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
 template <typename T, int V>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* __restrict__ logits, long long stride, int tokens,
                                                                  int experts, int top_k, bool normalize,
                                                                  float* __restrict__ weights, int* __restrict__ chosen) {
-  const int lane = threadIdx.x & 31;
-  const long long t = blockIdx.x * (long long)kRouteWarps + (threadIdx.x >> 5);
+  __shared__ uint2 room[kRouteWarps][32];
+  __shared__ float taken[kRouteWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long t = blockIdx.x * (long long)kRouteWarps + warp;
   if (t >= tokens) return;
   float x[V];
   load_scores<T, V>(logits + t * stride, experts, x);
-  float top, sum;
-  row_softmax<V>(x, top, sum);
+  float top = 0.f, sum = 0.f;
+  if (!normalize) row_softmax<V>(x, top, sum);
   bool nan = false;
-  uint32_t key[V];  // 0: off, or taken already
+  uint32_t key[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     nan = nan || x[v] != x[v];
     key[v] = x[v] > -INFINITY ? ordered(x[v]) : 0u;  // a NaN compares false
   }
   nan = __any_sync(0xffffffffu, nan);
-  int mine = -1;        // lane j: the j-th choice
-  float e_mine = 0.f;   // and its exp(x - top)
-  for (int j = 0; j < top_k; ++j) {
-    uint32_t best = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v) best = max(best, key[v]);
-    best = __reduce_max_sync(0xffffffffu, best);
-    if (best == 0) break;
-    int at = 0x7fffffff;
-#pragma unroll
-    for (int v = V - 1; v >= 0; --v)
-      if (key[v] == best) at = v * 32 + lane;
-    at = __reduce_min_sync(0xffffffffu, at);
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (at == v * 32 + lane) key[v] = 0;
-    if (lane == j) {
-      mine = at;
-      const uint32_t bits = best & 0x80000000u ? best & 0x7fffffffu : ~best;
-      e_mine = expf(__uint_as_float(bits) - top);
-    }
-  }
-  const float total = normalize ? warp_sum(e_mine) : sum;
+  const int found = top_keys<V>(key, top_k, room[warp], [&](int r, uint32_t k, int e) {
+    taken[warp][r] = unordered(k);
+    chosen[t * top_k + r] = e;
+  });
+  __syncwarp();
+  if (normalize) top = found > 0 ? taken[warp][0] : 0.f;
+  const float e = lane < found ? expf(taken[warp][lane] - top) : 0.f;
+  const float total = normalize ? warp_sum(e) : sum;
   if (lane < top_k) {
-    weights[t * top_k + lane] = mine < 0 ? 0.f : nan ? NAN : e_mine / total;
-    chosen[t * top_k + lane] = mine;
+    weights[t * top_k + lane] = lane >= found ? 0.f : nan ? NAN : e / total;
+    if (lane >= found) chosen[t * top_k + lane] = -1;
   }
 }
 
@@ -162,6 +218,7 @@ __global__ void __launch_bounds__(kSortThreads) expert_order(const void* __restr
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+  let_next_start();
   auto expert = [&](long long i) {
     const long long e = index_at(chosen, wide, i);
     return e >= 0 && e < experts ? int(e) : -1;
@@ -217,24 +274,18 @@ __device__ __forceinline__ void zero_blanks(const Blanks& b, int words, unsigned
     for (int c = lane; c < words; c += 32) reinterpret_cast<Word<B>*>(out + r * out_bytes)[c] = Word<B>{};
 }
 
+// A token's row to the rows of its choices, by `lanes` threads.
 template <int B>
-__global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsigned char* __restrict__ x, long long x_bytes,
-                                                                    const int* __restrict__ position, Blanks blanks, int tokens,
-                                                                    int top_k, int words, unsigned char* __restrict__ out,
-                                                                    long long out_bytes, int lanes_log2) {
-  if (int(blockIdx.x) < blanks.blocks()) return zero_blanks<B>(blanks, words, out, out_bytes);
-  const long long rows = blanks.rows;
-  const int lanes = 1 << lanes_log2;
-  const long long t = (blockIdx.x - blanks.blocks()) * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
-  if (t >= tokens) return;
-  const auto* src = reinterpret_cast<const Word<B>*>(x + t * x_bytes);
+__device__ __forceinline__ void copy_row(const unsigned char* x, const int* position, int top_k, long long rows, int words,
+                                         unsigned char* out, long long out_bytes, int lanes) {
+  const auto* src = reinterpret_cast<const Word<B>*>(x);
   for (int c = threadIdx.x & (lanes - 1); c < words; c += lanes * kRowUnroll) {
     Word<B> v[kRowUnroll];
 #pragma unroll
     for (int u = 0; u < kRowUnroll; ++u)
       if (c + u * lanes < words) v[u] = __ldg(src + c + u * lanes);
     for (int j = 0; j < top_k; ++j) {
-      const int p = position[t * top_k + j];
+      const int p = position[j];
       if (p < 0 || p >= rows) continue;
       auto* dst = reinterpret_cast<Word<B>*>(out + p * out_bytes);
 #pragma unroll
@@ -242,6 +293,92 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsign
         if (c + u * lanes < words) dst[c + u * lanes] = v[u];
     }
   }
+}
+
+// Few slots: one launch in which every block counts all of them for itself, instead
+// of a sort and a copy that waits for it.
+constexpr int kFewSlots = 2048;
+
+template <int B>
+__global__ void __launch_bounds__(kRowThreads) dispatch_few(const unsigned char* __restrict__ x, long long x_bytes,
+                                                            const void* __restrict__ chosen, bool wide, int n, int align,
+                                                            int* __restrict__ position, int* __restrict__ offsets,
+                                                            int* __restrict__ counts, Blanks blanks, int tokens, int top_k, int words,
+                                                            unsigned char* __restrict__ out, long long out_bytes, int lanes_log2) {
+  __shared__ int expert[kFewSlots], count[kMaxExperts], begin[kMaxExperts + 1], place[kRowThreads / 32 * kMaxTopK];
+  __shared__ int warp_total[kRowThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, experts = blanks.experts;
+  for (int e = threadIdx.x; e < experts; e += kRowThreads) count[e] = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < n; s += kRowThreads) {
+    const long long e = index_at(chosen, wide, s);
+    expert[s] = e >= 0 && e < experts ? int(e) : -1;
+    if (expert[s] >= 0) atomicAdd(count + expert[s], 1);
+  }
+  __syncthreads();
+  constexpr int kEach = kMaxExperts / kRowThreads;
+  int room[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = threadIdx.x * kEach + i;
+    room[i] = e < experts ? (count[e] + align - 1) / align * align : 0;
+    sum += room[i];
+  }
+  int before = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += o;
+  }
+  if (lane == 31) warp_total[warp] = before;
+  __syncthreads();
+  before -= sum;
+  for (int w = 0; w < warp; ++w) before += warp_total[w];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = threadIdx.x * kEach + i;
+    if (e <= experts) begin[e] = before;
+    before += room[i];
+  }
+  if (experts == kMaxExperts && threadIdx.x == kRowThreads - 1) begin[experts] = before;
+  __syncthreads();
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int e = threadIdx.x; e <= experts; e += kRowThreads) {
+      offsets[e] = begin[e];
+      if (e < experts) counts[e] = count[e];
+    }
+  }
+  if (int(blockIdx.x) < blanks.blocks()) {
+    blanks.offsets = begin;
+    blanks.counts = count;
+    return zero_blanks<B>(blanks, words, out, out_bytes);
+  }
+  const int lanes = 1 << lanes_log2;  // 32 at least
+  const int each = kRowThreads >> lanes_log2, first = (blockIdx.x - blanks.blocks()) * each;
+  for (int s = warp; s < each * top_k; s += kRowThreads / 32) {
+    const int slot = first * top_k + s;
+    if (slot >= n) break;
+    const int e = expert[slot];
+    int earlier = 0;
+    for (int i = lane; i < slot; i += 32) earlier += expert[i] == e;
+    earlier = __reduce_add_sync(0xffffffffu, earlier);
+    if (lane == 0) position[slot] = place[s] = e < 0 ? -1 : begin[e] + earlier;
+  }
+  __syncthreads();
+  const int own = threadIdx.x >> lanes_log2, t = first + own;
+  if (t < tokens) copy_row<B>(x + t * x_bytes, place + own * top_k, top_k, blanks.rows, words, out, out_bytes, lanes);
+}
+
+template <int B>
+__global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsigned char* __restrict__ x, long long x_bytes,
+                                                                    const int* position, Blanks blanks, int tokens, int top_k,
+                                                                    int words, unsigned char* __restrict__ out,
+                                                                    long long out_bytes, int lanes_log2) {
+  wait_for_previous();
+  if (int(blockIdx.x) < blanks.blocks()) return zero_blanks<B>(blanks, words, out, out_bytes);
+  const long long t = (blockIdx.x - blanks.blocks()) * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
+  if (t < tokens)
+    copy_row<B>(x + t * x_bytes, position + t * top_k, top_k, blanks.rows, words, out, out_bytes, 1 << lanes_log2);
 }
 
 template <typename T, int N, int W, bool kWeighted>
@@ -413,19 +550,26 @@ long long dispatch_rows(long long slots, int experts, int align) {
 void dispatch_launch(int dtype, RowsIn x, Indices chosen, int tokens, int top_k, int experts, int align, int width, RowsOut out,
                      long long row_count, bool zero_tail, int* position, int* offsets, int* counts, cudaStream_t stream) {
   const long long n = chosen.count;
-  launch_clusters<expert_order>(sort_blocks(n), 1, experts, stream, chosen.ptr, chosen.wide, n, experts, align, position, offsets,
-                                counts);
   const Blanks blanks{offsets, counts, row_count, experts, tail_blocks(zero_tail, row_count), align > 1 ? experts * kPadBlocks : 0};
-  if (n == 0 && blanks.tail == 0) return;
   const int size = dtype_size(dtype);
   const long long row_bytes = (long long)width * size;
+  const bool few = n <= kFewSlots;
+  if (!few)
+    launch_clusters<expert_order>(sort_blocks(n), 1, experts, stream, chosen.ptr, chosen.wide, n, experts, align, position, offsets,
+                                  counts);
   auto run = [&](auto bytes) {
     constexpr int B = decltype(bytes)::value;
-    const int words = int(row_bytes / B), lanes_log2 = row_lanes(words, kRowUnroll, 0);
-    const unsigned blocks = grid_x(blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2));
-    dispatch_rows_kernel<B><<<blocks, kRowThreads, 0, stream>>>(
-        static_cast<const unsigned char*>(x.ptr), x.stride * size, position, blanks, tokens, top_k, words,
-        static_cast<unsigned char*>(out.ptr), out.stride * size, lanes_log2);
+    const auto* src = static_cast<const unsigned char*>(x.ptr);
+    auto* dst = static_cast<unsigned char*>(out.ptr);
+    const int words = int(row_bytes / B), lanes_log2 = few ? row_lanes(words, 1, 5) : row_lanes(words, kRowUnroll, 0);
+    const long long blocks = blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2);
+    if (few)
+      dispatch_few<B><<<grid_x(std::max(1LL, blocks)), kRowThreads, 0, stream>>>(
+          src, x.stride * size, chosen.ptr, chosen.wide, int(n), align, position, offsets, counts, blanks, tokens, top_k, words, dst,
+          out.stride * size, lanes_log2);
+    else
+      launch_after(dispatch_rows_kernel<B>, grid_x(blocks), kRowThreads, stream, src, x.stride * size, position, blanks, tokens,
+                   top_k, words, dst, out.stride * size, lanes_log2);
   };
   auto fits = [&](int bytes) {
     return row_bytes % bytes == 0 && rows_aligned(x.ptr, x.stride, size, bytes) && rows_aligned(out.ptr, out.stride, size, bytes);

@@ -27,8 +27,9 @@ namespace psb {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kMaxDigits = 1024;  // one thread a digit
+constexpr int kMaxBits = 10, kMaxDigits = 1 << kMaxBits;  // one thread a digit
 constexpr int kKeep = 8;
+constexpr int kSortBlocks = 8;     // the largest cluster that needs no opt-in
 
 struct Strip {
   long long begin, end;
@@ -43,10 +44,20 @@ __device__ __forceinline__ Strip warp_strip(long long n, int rank, int blocks) {
 }
 
 // row[d] of the lanes' digits d (-1: none) before this chunk of 32, plus the number of
-// lower lanes of the same digit; row[d] is counted up.
-__device__ __forceinline__ uint32_t rank_chunk(uint32_t* row, int d) {
+// lower lanes of the same digit; row[d] is counted up.  The lanes of equal digit are
+// found with a ballot for each of the digit's `bits`: __match_any_sync gives them in
+// one call, but an SM answers one in 58 cycles (65536 indices, 64 digits: 15.0k cycles
+// of a pass go into the ranks, 8.8k with ballots).
+__device__ __forceinline__ uint32_t rank_chunk(uint32_t* row, int d, int bits) {
   const int lane = threadIdx.x & 31;
-  const unsigned same = __match_any_sync(0xffffffffu, d);
+  unsigned same = __ballot_sync(0xffffffffu, d >= 0);
+#pragma unroll
+  for (int b = 0; b < kMaxBits; ++b) {
+    if (b >= bits) break;
+    const bool set = d & (1 << b);
+    const unsigned with = __ballot_sync(0xffffffffu, set);
+    same &= set ? with : ~with;
+  }
   const uint32_t first = d >= 0 ? row[d] : 0u;
   __syncwarp();
   if (d >= 0 && lane == __ffs(same) - 1) row[d] = first + __popc(same);
@@ -79,31 +90,31 @@ __device__ __forceinline__ uint32_t block_sum_before(uint32_t v, uint32_t* scrat
   return scratch[warp] + inc - v;
 }
 
-// Shared memory of a sort: kSortWarps rows of counters (an odd pitch, so that a warp
-// reads a column without bank conflicts), two sets of block totals (one pass writes
-// one while a slower block may still read the other), the digits' bases and scratch.
+// The cluster's barrier; a cluster of one block needs only the block's.
+__device__ __forceinline__ void sort_barrier(int blocks) {
+  if (blocks == 1) __syncthreads();
+  else cooperative_groups::this_cluster().sync();
+}
+
+// Shared memory of a sort: kSortWarps rows of counters, two sets of block totals (one
+// pass writes one while a slower block may still read the other), the digits' bases
+// and scratch.
 struct SortShared {
   uint32_t* rows;
   uint32_t* total;
   uint32_t* base;
   uint32_t* scratch;
-  int pitch;
   __device__ SortShared(uint32_t* smem, int digits)
-      : rows(smem),
-        total(smem + kSortWarps * (digits | 1)),
-        base(total + 2 * digits),
-        scratch(base + digits),
-        pitch(digits | 1) {}
+      : rows(smem), total(smem + kSortWarps * digits), base(total + 2 * digits), scratch(base + digits) {}
 };
-inline size_t sort_smem(int digits) {
-  return sizeof(uint32_t) * (size_t(kSortWarps) * (digits | 1) + 3 * size_t(digits) + kSortWarps);
-}
+inline size_t sort_smem(int digits) { return sizeof(uint32_t) * ((kSortWarps + 3) * size_t(digits) + kSortWarps); }
 
 // One pass: place(i, element, p) for every element of the strip, p its position in the
 // stable order by digit.  load(i) gives the element i, digit_of(element) its digit (-1:
 // the element is not counted, and p means nothing).  widen(count) is the room that the
 // elements of a digit take (at least count); report(d, begin, count) is called by one
-// thread a digit in every block.  Ends with the cluster's barrier.
+// thread a digit in every block.  digits <= kMaxDigits.  Ends with the
+// cluster's barrier.
 template <typename Element, typename Load, typename DigitOf, typename Widen, typename Report, typename Place>
 __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity, Strip strip, Load&& load, DigitOf&& digit_of,
                                           Widen&& widen, Report&& report, Place&& place) {
@@ -111,7 +122,8 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t* row = sh.rows + warp * sh.pitch;
+  const int bits = 32 - __clz(digits - 1);
+  uint32_t* row = sh.rows + warp * digits;
   for (int d = lane; d < digits; d += 32) row[d] = 0;
   __syncwarp();
 
@@ -126,29 +138,34 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
     }
 #pragma unroll
     for (int u = 0; u < kKeep; ++u)
-      if (base + u * 32 < strip.end) r[u] = rank_chunk(row, base + u * 32 + lane < strip.end ? digit_of(e[u]) : -1);
+      if (base + u * 32 < strip.end) r[u] = rank_chunk(row, base + u * 32 + lane < strip.end ? digit_of(e[u]) : -1, bits);
   }
   __syncthreads();
 
-  // Counts to positions within the block: a warp takes every kSortWarps-th digit, a lane
-  // the counter of one warp.
-  for (int d = warp; d < digits; d += kSortWarps) {
-    const uint32_t c = sh.rows[lane * sh.pitch + d];
-    uint32_t inc = c;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, inc, s);
-      if (lane >= s) inc += o;
-    }
-    sh.rows[lane * sh.pitch + d] = inc - c;
-    if (lane == 31) sh.total[parity * digits + d] = inc;
-  }
-  cluster.sync();
-
+  // Counts to positions within the block, a thread a digit.
   const int d = threadIdx.x;
+  if (d < digits) {
+    uint32_t sum = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWarps; w += 16) {
+      uint32_t c[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) c[k] = sh.rows[(w + k) * digits + d];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        sh.rows[(w + k) * digits + d] = sum;
+        sum += c[k];
+      }
+    }
+    sh.total[parity * digits + d] = sum;
+  }
+  sort_barrier(blocks);
+
   uint32_t count = 0, earlier = 0;
   if (d < digits) {
-    for (int b = 0; b < blocks; ++b) {
+#pragma unroll
+    for (int b = 0; b < kSortBlocks; ++b) {
+      if (b >= blocks) break;
       const uint32_t c = cluster.map_shared_rank(sh.total, b)[parity * digits + d];
       if (b < rank) earlier += c;
       count += c;
@@ -182,19 +199,41 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
         if (base + u * 32 >= strip.end) break;
         const long long i = base + u * 32 + lane;
         const int digit = i < strip.end ? digit_of(e[u]) : -1;
-        const uint32_t p = rank_chunk(row, digit);
+        const uint32_t p = rank_chunk(row, digit, bits);
         if (i < strip.end) place(i, e[u], digit < 0 ? 0u : sh.base[digit] + p);
       }
     }
   }
   // The places are visible to the cluster, and no block ends (or counts again) while
   // another may read its totals.
-  cluster.sync();
+  sort_barrier(blocks);
 }
 
 // Blocks of the cluster for n indices: one while each warp's strip is short, more as
-// the strips grow (8 is the largest cluster that needs no opt-in).
-inline int sort_blocks(long long n) { return n <= 2048 ? 1 : n <= 8192 ? 4 : 8; }
+// the strips grow.
+inline int sort_blocks(long long n) { return n <= 2048 ? 1 : n <= 8192 ? 4 : kSortBlocks; }
+
+// A kernel launched with launch_after may start while the one before it still runs; it
+// waits here before it touches what that one writes, and reads that with plain loads
+// (the read-only path may hold lines from before the wait).  let_next_start() in the earlier
+// kernel lets the later one's blocks take their places as soon as every block of the
+// earlier one has its own.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+void launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.stream = stream;
+  cudaLaunchAttribute attr[1] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  PSB_CUDA(cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...));
+}
 
 // Launches `kernel` with `clusters` clusters of `blocks` blocks of kSortThreads.
 template <auto kernel, typename... Args>
