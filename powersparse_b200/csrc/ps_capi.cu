@@ -326,7 +326,8 @@ int ps_embedding_grad(const void* grad, int grad_dtype, long long grad_stride, c
     require(rows >= 1 && rows < 0x7fffffffLL, what, "the table's rows must be in [1, 2^31 - 2]");
     require_rows(grad, grad_stride, n, width, in_size, what);
     require_rows(grad_table, table_stride, rows, width, out_size, what);
-    require(workspace_bytes >= (long long)psb::embedding_grad_workspace(n, width) && workspace != nullptr, what,
+    const long long need = (long long)psb::embedding_grad_workspace(n, width);
+    require(workspace_bytes >= need && (workspace != nullptr || need == 0), what,
             "the workspace is smaller than ps_embedding_grad_workspace says");
     require(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, what, "the workspace must begin at a multiple of 256 bytes");
     psb::embedding_grad_launch(grad_dtype, {grad, grad_stride}, index, scale, padding, accumulate != 0, table_dtype,

@@ -93,7 +93,7 @@ struct Clear {
 // since the sort leaves most of the GPU idle.
 __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __restrict__ tokens, bool wide, long long n,
                                                                 long long rows, long long padding, int pass_bits, int passes,
-                                                                Item* a, Item* b, int chunk, int* joins, int* join_count,
+                                                                Item* a, Item* b, int chunk, Item* joins, int* join_count,
                                                                 Clear zeros) {
   extern __shared__ uint32_t smem[];
   namespace cg = cooperative_groups;
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
   for (long long c = rank * kSortThreads + threadIdx.x; (c + 1) * chunk < n; c += blocks * kSortThreads) {
     const uint32_t token = a[(c + 1) * chunk - 1].token;
     if (token < rows && a[(c + 1) * chunk].token == token && (c == 0 || a[c * chunk - 1].token != token))
-      joins[atomicAdd(join_count, 1)] = int(c);
+      joins[atomicAdd(join_count, 1)] = {token, uint32_t(c)};
   }
 }
 
@@ -201,28 +201,29 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
   }
 }
 
-// The runs that cross a border, by the list of the chunks in which they begin: their
-// partial rows, added in order by each of the block's warps (every kJoinWarps-th chunk)
-// and then over the warps.
+// The runs that cross a border, by the list of their tokens and the chunks in which
+// they begin: their partial rows, added in order by each of the block's warps (every
+// kJoinWarps-th chunk) and then over the warps.
 constexpr int kJoinWarps = 8;
 
 template <typename O, int N, int W>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, long long n, int width, float scale,
                                                              bool accumulate, O* __restrict__ out, long long out_stride, int chunk,
-                                                             const float* partial, const int* joins, const int* join_count) {
+                                                             const float* partial, const Item* joins, const int* join_count,
+                                                             long long most) {
   __shared__ float sums[kJoinWarps][32 * N];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slabs = ceil_div(width, 32 * N);
   wait_for_previous();
-  const long long work = (long long)*join_count * slabs;
-  for (long long item = blockIdx.x; item < work; item += gridDim.x) {
-    const long long own = joins[item / slabs];
-    const int c = int(item % slabs) * 32 * N + lane * W;
-    const uint32_t token = items[(own + 1) * chunk - 1].token;
+  for (long long i = blockIdx.x; i < most; i += gridDim.x) {
+    const Item join = joins[i / slabs];  // read beside the count, not after it: there is room for `most`
+    if (i >= (long long)*join_count * slabs) return;
+    const int c = int(i % slabs) * 32 * N + lane * W;
+    const long long own = join.place;
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
-    for (long long j = own + warp; j * chunk < n && (j == own || items[j * chunk].token == token); j += kJoinWarps) {
+    for (long long j = own + warp; j * chunk < n && (j == own || items[j * chunk].token == join.token); j += kJoinWarps) {
       if (c < width) {
         Pack<float, N, W> v;
         v.zero();
@@ -238,13 +239,131 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, 
       for (int w = 1; w < kJoinWarps; ++w)
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] += sums[w][e * 32 + lane];
-      write_sum<O, N, W>(out + (long long)token * out_stride, c, 32 * W, width, acc, scale, accumulate);
+      write_sum<O, N, W>(out + (long long)join.token * out_stride, c, 32 * W, width, acc, scale, accumulate);
     }
     __syncthreads();
   }
 }
 
-int chunk_of(long long n) { return n >= 16384 ? 32 : n >= 2048 ? 16 : 4; }
+// ---- gradient of few tokens: one launch ---------------------------------------------
+// A block for every token of the batch: the first of its kind adds up all of them (the
+// others end), in the order of the batch.  Up to kFewTokens / kFewThreads tokens a
+// thread are compared, so no sort is needed, and neither are partial rows.  Behind them
+// the blocks that clear the rows which no token names.
+constexpr int kFewTokens = 2048;
+constexpr int kFewThreads = 256;
+constexpr int kFewEach = kFewTokens / kFewThreads;
+constexpr int kFewWarps = kFewThreads / 32;
+constexpr int kLongRun = 64;         // from here on a block's warps share out the rows, not the columns
+constexpr int kClearRows = 4096;     // rows a clearing block takes at the most,
+constexpr int kClearBytes = 1 << 16; // and about so many bytes
+
+// The thread's tokens threadIdx.x + k * kFewThreads as rows of the table (-1: none).
+__device__ __forceinline__ void few_tokens(const void* tokens, bool wide, int n, long long rows, long long padding,
+                                           int (&v)[kFewEach]) {
+#pragma unroll
+  for (int k = 0; k < kFewEach; ++k) {
+    const int i = threadIdx.x + k * kFewThreads;
+    const long long t = i < n ? index_at(tokens, wide, i) : -1;
+    v[k] = t >= 0 && t < rows && t != padding ? int(t) : -1;
+  }
+}
+
+template <typename T, typename O, int N, int W>
+__global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ grad, long long grad_stride,
+                                                       const void* __restrict__ tokens, bool wide, int n, long long rows,
+                                                       long long padding, int width, float scale, bool accumulate,
+                                                       O* __restrict__ out, long long out_stride, int clear_rows, int lanes_log2) {
+  __shared__ union {
+    struct {
+      unsigned short list[kFewTokens];
+      int count[kFewEach * kFewWarps];
+      float sums[N][kFewThreads];
+    };
+    unsigned char touched[kClearRows];
+  } sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int v[kFewEach];
+  if (int(blockIdx.x) >= n) {
+    const long long first = (long long)(blockIdx.x - n) * clear_rows;
+    few_tokens(tokens, wide, n, rows, padding, v);
+    for (int r = threadIdx.x; r < clear_rows; r += kFewThreads) sh.touched[r] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kFewEach; ++k)
+      if (v[k] >= first && v[k] < first + clear_rows) sh.touched[v[k] - first] = 1;
+    __syncthreads();
+    const int lanes = 1 << lanes_log2;
+    for (int r = threadIdx.x >> lanes_log2; r < clear_rows && first + r < rows; r += kFewThreads >> lanes_log2)
+      if (!sh.touched[r])
+        clear(reinterpret_cast<unsigned char*>(out + (first + r) * out_stride), (long long)width * sizeof(O),
+              threadIdx.x & (lanes - 1), lanes);
+    return;
+  }
+  const int own = blockIdx.x;
+  const long long token = index_at(tokens, wide, own);
+  if (token < 0 || token >= rows || token == padding) return;
+  few_tokens(tokens, wide, n, rows, padding, v);
+  bool earlier = false;
+  unsigned same[kFewEach];
+#pragma unroll
+  for (int k = 0; k < kFewEach; ++k) {
+    const bool match = v[k] == int(token);
+    earlier = earlier || (match && int(threadIdx.x) + k * kFewThreads < own);
+    same[k] = __ballot_sync(0xffffffffu, match);
+    if (lane == 0) sh.count[k * kFewWarps + warp] = __popc(same[k]);
+  }
+  if (__syncthreads_or(earlier)) return;
+  // Places of the matches in order: threads' words are in the order of k, then warp, then lane.
+  int total = 0, before[kFewEach];
+#pragma unroll
+  for (int k = 0; k < kFewEach; ++k)
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      if (w == warp) before[k] = total;
+      total += sh.count[k * kFewWarps + w];
+    }
+#pragma unroll
+  for (int k = 0; k < kFewEach; ++k)
+    if (same[k] >> lane & 1)
+      sh.list[before[k] + __popc(same[k] & ((1u << lane) - 1u))] = (unsigned short)(threadIdx.x + k * kFewThreads);
+  __syncthreads();
+
+  constexpr int kUnroll = 4;
+  const int lanes = total > kLongRun ? 32 : 1 << lanes_log2, groups = kFewThreads / lanes;  // threads a row, rows at a time
+  const int group = threadIdx.x / lanes, step = lanes * W;
+  for (int slab = 0; slab < width; slab += lanes * N) {
+    const int c = slab + (threadIdx.x & (lanes - 1)) * W;
+    float acc[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.f;
+    for (int i = group; i < total; i += groups * kUnroll) {
+      Pack<T, N, W> x[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        x[u].zero();
+        if (i + u * groups < total) x[u].load(grad + sh.list[i + u * groups] * grad_stride, c, step, width);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += x[u].get(e);
+    }
+    if (groups > 1) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) sh.sums[e][threadIdx.x] = acc[e];
+      __syncthreads();
+      if (group == 0)
+        for (int g = 1; g < groups && g < total; ++g)
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[e] += sh.sums[e][g * lanes + threadIdx.x];
+      __syncthreads();
+    }
+    if (group == 0) write_sum<O, N, W>(out + token * out_stride, c, step, width, acc, scale, accumulate);
+  }
+}
+
+int chunk_of(long long n) { return n >= 16384 ? 32 : 16; }
 
 constexpr size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -256,7 +375,7 @@ struct Workspace {
     b = a + align_up(size_t(n) * sizeof(Item));
     join_count = b + align_up(size_t(n) * sizeof(Item));
     joins = join_count + align_up(sizeof(int));
-    partial = joins + align_up(size_t(chunks) * sizeof(int));
+    partial = joins + align_up(size_t(chunks) * sizeof(Item));
     bytes = partial + align_up(size_t(chunks) * 2 * size_t(width) * sizeof(float));
   }
 };
@@ -284,7 +403,7 @@ void embedding_launch(int dtype, RowsIn table, long long rows, int width, Indice
   PSB_LAUNCH_CHECK();
 }
 
-size_t embedding_grad_workspace(long long tokens, int width) { return Workspace(tokens, width).bytes; }
+size_t embedding_grad_workspace(long long tokens, int width) { return tokens <= kFewTokens ? 0 : Workspace(tokens, width).bytes; }
 
 void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float scale, long long padding, bool accumulate,
                            int out_dtype, RowsOut out, long long rows, int width, void* workspace, cudaStream_t stream) {
@@ -294,18 +413,19 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
   const Workspace at(n, width);
   char* ws = static_cast<char*>(workspace);
   auto* items = reinterpret_cast<Item*>(ws + at.a);
-  auto* joins = reinterpret_cast<int*>(ws + at.joins);
+  auto* joins = reinterpret_cast<Item*>(ws + at.joins);
   auto* join_count = reinterpret_cast<int*>(ws + at.join_count);
   auto* partial = reinterpret_cast<float*>(ws + at.partial);
-  {
-    const Clear zeros(out.ptr, rows, (long long)width * out_size, out.stride * out_size);
-    const int bits = bits_for((unsigned long long)rows), passes = ceil_div(bits, 10), pass_bits = ceil_div(bits, passes);
+  const bool few = n <= kFewTokens;
+  const long long row_bytes = (long long)width * out_size;
+  if (!few) {
+    const Clear zeros(out.ptr, rows, row_bytes, out.stride * out_size);
+    const int bits = bits_for((unsigned long long)rows), passes = ceil_div(bits, kMaxBits), pass_bits = ceil_div(bits, passes);
     const int blocks = sort_blocks(n);
     const long long clusters = 1 + (accumulate ? 0 : ceil_div_ll(zeros.blocks(), blocks));
     launch_clusters<embedding_order>(blocks, clusters, 1 << pass_bits, stream, tokens.ptr, tokens.wide, n, rows, padding, pass_bits,
                                      passes, items, reinterpret_cast<Item*>(ws + at.b), chunk, joins, join_count, zeros);
   }
-  if (n == 0) return;
   auto run = [&](auto t, auto o) {
     using T = decltype(t);
     using O = decltype(o);
@@ -315,14 +435,23 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
     with_shape<T>(width, fits, [&](auto shape) {
       constexpr int N = decltype(shape)::N, W = decltype(shape)::W;
       O* dst = static_cast<O*>(out.ptr);
+      if (few) {
+        const int clear_rows = int(std::min<long long>(kClearRows, std::max<long long>(1, kClearBytes / row_bytes)));
+        const long long blocks = n + (accumulate ? 0 : ceil_div_ll(rows, clear_rows));  // n and blocks are not both 0
+        sum_few<T, O, N, W><<<grid_x(blocks), kFewThreads, 0, stream>>>(
+            static_cast<const T*>(grad.ptr), grad.stride, tokens.ptr, tokens.wide, int(n), rows, padding, width, scale, accumulate,
+            dst, out.stride, clear_rows, row_lanes(ceil_div(width, N), 1, 2));
+        PSB_LAUNCH_CHECK();
+        return;
+      }
       const unsigned chunks = grid_x(ceil_div_ll(n, chunk));
       const dim3 sums(chunks, unsigned(ceil_div(width, kSumThreads * N)));
       launch_after(sum_runs<T, O, N, W>, sums, kSumThreads, stream, static_cast<const T*>(grad.ptr), grad.stride, items, n,
                    uint32_t(rows), width, scale, accumulate, dst, out.stride, chunk, partial);
       if (chunks == 1) return;
-      const long long work = (long long)(chunks - 1) * ceil_div(width, 32 * N);
-      launch_after(join_runs<O, N, W>, unsigned(std::min<long long>(work, 4LL * device_sms())), kJoinWarps * 32, stream, items, n,
-                   width, scale, accumulate, dst, out.stride, chunk, partial, joins, join_count);
+      const long long most = (long long)(chunks - 1) * ceil_div(width, 32 * N);
+      launch_after(join_runs<O, N, W>, unsigned(std::min<long long>(most, 8LL * device_sms())), kJoinWarps * 32, stream, items, n,
+                   width, scale, accumulate, dst, out.stride, chunk, partial, joins, join_count, most);
     });
   };
   with_type(grad_dtype, [&](auto t) {

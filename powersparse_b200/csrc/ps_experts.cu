@@ -21,139 +21,154 @@ namespace psb {
 namespace {
 
 // ---- router -----------------------------------------------------------------------
-// A warp a token, E / 32 scores a lane in registers.  Scores compare as integers that
-// keep the order of the numbers (-0 as +0); of equal scores the lowest index comes
-// first.  A score of -inf switches an expert off: it is never chosen.
+// A warp a token; lane l holds the V scores from l * V on in registers, so that a lane
+// loads words of 16 bytes where the rows allow it (`words`) and the lanes' order is the
+// experts'.  Scores compare as numbers: -0 equals +0, a NaN compares false and is never
+// chosen, and -inf (off) lies below kLowest, the least score that can be.  Of equal
+// scores the lowest index comes first.
 constexpr int kRouteWarps = 8;
+constexpr float kLowest = -3.402823466e+38f;
 
-__device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t b = __float_as_uint(x + 0.f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
 }
 
+// Scores a load: all of a lane's, up to 16 bytes.
 template <typename T, int V>
-__device__ __forceinline__ void load_scores(const T* row, int experts, float (&x)[V]) {
-  const int lane = threadIdx.x & 31;
+constexpr int kScoreWord = V * int(sizeof(T)) < 16 ? V : 16 / int(sizeof(T));
+
+// A lane's scores, -inf behind the last expert.
+template <typename T, int V>
+__device__ __forceinline__ void load_scores(Pack<T, V, kScoreWord<T, V>>& p, const T* row, int c, int step, int experts, bool words) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = v * 32 + lane;
-    x[v] = e < experts ? to_float(row[e]) : -INFINITY;
-  }
+  for (int v = 0; v < V; ++v) p.set(v, -INFINITY);
+  if (words) p.load(row, c, step, experts);
+  else p.load_elements(row, c, step, experts);
 }
 
-// Largest score of the row (0 where all are -inf, so that x - max is not NaN), and
-// the sum of exp(x - max) over the row.
-template <int V>
-__device__ __forceinline__ void row_softmax(const float (&x)[V], float& top, float& sum) {
-  top = -INFINITY;
-#pragma unroll
-  for (int v = 0; v < V; ++v) top = fmaxf(top, x[v]);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (top == -INFINITY) top = 0.f;
-  sum = 0.f;
-#pragma unroll
-  for (int v = 0; v < V; ++v) sum += expf(x[v] - top);
-  sum = warp_sum(sum);
-}
+struct Gathered {
+  float2 item[32];  // score and index
+  float taken[32];  // scores by rank
+};
 
-// The top_k largest of a warp's keys (0: never taken), ranked: take(r, key, index) is
-// called by one lane for every rank r that there is; returns their number.
+// The top_k largest of a warp's scores, ranked: g.taken[r] is the score of rank r and
+// take(r, index) is called by one lane for every rank r that there is; returns their
+// number and sets `top` to the largest (kLowest where there is none).
 //
-// The k-th largest of the 32 lanes' own maxima is a bound that at least k keys reach,
-// and rarely many more do: those are gathered in shared memory and each lane ranks one
-// of them among all.  Where more than 32 reach it (equal scores), the keys are taken
-// one by one instead, as they are for few choices, where that is faster.
-constexpr int kTakeOneByOne = 3;
-
+// The k-th largest of the 32 lanes' own maxima is a bound that at least k scores reach,
+// and rarely many more do: those are gathered in shared memory, where each lane ranks
+// one of them among all.  Where more than 32 reach it (equal scores), the scores are
+// taken one by one instead.  What bounds it is the instructions: 16384 tokens of 256
+// experts, top 8, took 17.0 us with a maximum over the warp for each choice and take
+// 7.3 us so.
 template <int V, typename Take>
-__device__ __forceinline__ int top_keys(uint32_t (&key)[V], int top_k, uint2* room, Take&& take) {
+__device__ __forceinline__ int top_scores(float (&x)[V], int top_k, Gathered& g, float& top, Take&& take) {
   const int lane = threadIdx.x & 31;
-  uint32_t best = 0;
+  float best = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < V; ++v) best = max(best, key[v]);
-  if (top_k > kTakeOneByOne) {
-    uint32_t sorted = best;  // bitonic, largest first
+  for (int v = 0; v < V; ++v) best = fmaxf(best, x[v]);
+  float sorted = best;  // bitonic, largest first
 #pragma unroll
-    for (int size = 2; size <= 32; size *= 2)
+  for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
-      for (int stride = size / 2; stride > 0; stride /= 2) {
-        const uint32_t other = __shfl_xor_sync(0xffffffffu, sorted, stride);
-        const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
-        sorted = larger ? max(sorted, other) : min(sorted, other);
-      }
-    const uint32_t bound = max(1u, __shfl_sync(0xffffffffu, sorted, top_k - 1));
-    int found = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const unsigned reach = __ballot_sync(0xffffffffu, key[v] >= bound);
-      const int slot = found + __popc(reach & ((1u << lane) - 1u));
-      if (key[v] >= bound && slot < 32) room[slot] = make_uint2(key[v], v * 32 + lane);
-      found += __popc(reach);
+    for (int stride = size / 2; stride > 0; stride /= 2) {
+      const float other = __shfl_xor_sync(0xffffffffu, sorted, stride);
+      const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
+      sorted = larger ? fmaxf(sorted, other) : fminf(sorted, other);
     }
-    if (found <= 32) {
-      __syncwarp();
-      const uint2 mine = lane < found ? room[lane] : make_uint2(0, 0);
-      int rank = 0;  // the slots ascend with the index: of equal keys the lower slot first
-      for (int i = 0; i < found; ++i) {
-        const uint32_t other = room[i].x;
-        rank += other > mine.x || (other == mine.x && i < lane);
-      }
-      if (lane < found && rank < top_k) take(rank, mine.x, int(mine.y));
-      return min(found, top_k);
+  top = fmaxf(kLowest, __shfl_sync(0xffffffffu, sorted, 0));
+  const float bound = fmaxf(kLowest, __shfl_sync(0xffffffffu, sorted, top_k - 1));
+  int mine = 0;
+#pragma unroll
+  for (int v = 0; v < V; ++v) mine += x[v] >= bound;
+  int slot = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, slot, d);
+    if (lane >= d) slot += o;
+  }
+  const int found = __shfl_sync(0xffffffffu, slot, 31);
+  if (found <= 32) {
+    slot -= mine;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (x[v] >= bound) g.item[slot++] = make_float2(x[v], __int_as_float(lane * V + v));
+    if (lane >= found) g.item[lane] = make_float2(-INFINITY, 0.f);
+    __syncwarp();
+    const float2 own = g.item[lane];
+    int rank = 0;
+    for (int i = 0; i < found; i += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(g.item + i), b = *reinterpret_cast<const float4*>(g.item + i + 2);
+      rank += (a.x > own.x) + (a.z > own.x) + (b.x > own.x) + (b.z > own.x);
     }
+    // Equal scores have got the same rank, so the ranks add up to less than they should:
+    // then, as the slots ascend with the index, the lower slot comes first.
+    if (__reduce_add_sync(0xffffffffu, lane < found ? rank : 0) != found * (found - 1) / 2)
+      for (int i = 0; i < found; ++i) rank += g.item[i].x == own.x && i < lane;
+    if (lane < found && rank < top_k) {
+      g.taken[rank] = own.x;
+      take(rank, __float_as_int(own.y));
+    }
+    return min(found, top_k);
   }
   for (int j = 0; j < top_k; ++j) {
-    const uint32_t largest = __reduce_max_sync(0xffffffffu, best);
-    if (largest == 0) return j;
+    const float largest = warp_max(best);
+    if (!(largest >= kLowest)) return j;
     int at = 0x7fffffff;
 #pragma unroll
     for (int v = V - 1; v >= 0; --v)
-      if (key[v] == largest) at = v * 32 + lane;
+      if (x[v] == largest) at = lane * V + v;
     const int first = __reduce_min_sync(0xffffffffu, at);
-    best = 0;
+    best = -INFINITY;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      if (first == v * 32 + lane) key[v] = 0;
-      best = max(best, key[v]);
+      if (first == lane * V + v) x[v] = -INFINITY;
+      best = fmaxf(best, x[v]);
     }
-    if (at == first) take(j, largest, first);
+    if (at == first) {
+      g.taken[j] = largest;
+      take(j, first);
+    }
   }
   return top_k;
 }
 
-__device__ __forceinline__ float unordered(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
-
 template <typename T, int V>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* __restrict__ logits, long long stride, int tokens,
-                                                                 int experts, int top_k, bool normalize,
+__global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* __restrict__ logits, long long stride, bool words,
+                                                                 int tokens, int experts, int top_k, bool normalize,
                                                                  float* __restrict__ weights, int* __restrict__ chosen) {
-  __shared__ uint2 room[kRouteWarps][32];
-  __shared__ float taken[kRouteWarps][32];
+  __shared__ __align__(16) Gathered gathered[kRouteWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long t = blockIdx.x * (long long)kRouteWarps + warp;
   if (t >= tokens) return;
-  float x[V];
-  load_scores<T, V>(logits + t * stride, experts, x);
-  float top = 0.f, sum = 0.f;
-  if (!normalize) row_softmax<V>(x, top, sum);
+  float x[V], top;
   bool nan = false;
-  uint32_t key[V];
+  {
+    Pack<T, V, kScoreWord<T, V>> p;
+    load_scores<T, V>(p, logits + t * stride, lane * V, kScoreWord<T, V>, experts, words);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    nan = nan || x[v] != x[v];
-    key[v] = x[v] > -INFINITY ? ordered(x[v]) : 0u;  // a NaN compares false
+    for (int v = 0; v < V; ++v) {
+      x[v] = p.get(v);
+      nan = nan || x[v] != x[v];
+    }
   }
   nan = __any_sync(0xffffffffu, nan);
-  const int found = top_keys<V>(key, top_k, room[warp], [&](int r, uint32_t k, int e) {
-    taken[warp][r] = unordered(k);
-    chosen[t * top_k + r] = e;
-  });
+  float sum = 0.f;
+  if (!normalize) {
+    top = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < V; ++v) top = fmaxf(top, x[v]);
+    top = fmaxf(kLowest, warp_max(top));
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += expf(x[v] - top);
+    sum = warp_sum(sum);
+  }
+  Gathered& g = gathered[warp];
+  const int found = top_scores<V>(x, top_k, g, top, [&](int r, int e) { chosen[t * top_k + r] = e; });
   __syncwarp();
-  if (normalize) top = found > 0 ? taken[warp][0] : 0.f;
-  const float e = lane < found ? expf(taken[warp][lane] - top) : 0.f;
+  const float e = lane < found ? expf(g.taken[lane] - top) : 0.f;
   const float total = normalize ? warp_sum(e) : sum;
   if (lane < top_k) {
     weights[t * top_k + lane] = lane >= found ? 0.f : nan ? NAN : e / total;
@@ -161,53 +176,66 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* __rest
   }
 }
 
-// With p the softmax that the weights are shares of, and G = sum_j g_j w_j:
-//   d logits[e] = p[e] * (g of the choice e, or 0) - p[e] * G.
+// With p the softmax that the weights are shares of, g[e] the gradient of the choice e (0
+// where it was not chosen) and G = sum_j g_j w_j:  d logits[e] = p[e] * (g[e] - G).
 // Shares of all experts: p from the logits, dense.  Shares of the chosen ones
-// (normalize): p is the weights, zero elsewhere, and the logits are not read.
+// (normalize): p is the weights, zero elsewhere, and the logits are not read.  g (or
+// w_j (g_j - G)) is spread over the experts in shared memory.  A lane's words stand 32
+// words apart, so that a warp writes whole sectors.
 template <typename T, int V, bool kNormalize>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const float* __restrict__ grad, const T* __restrict__ logits,
-                                                                      long long stride, const float* __restrict__ weights,
+                                                                      long long stride, bool words, const float* __restrict__ weights,
                                                                       const int* __restrict__ chosen, int tokens, int experts,
                                                                       int top_k, T* __restrict__ out, long long out_stride) {
-  const int lane = threadIdx.x & 31;
-  const long long t = blockIdx.x * (long long)kRouteWarps + (threadIdx.x >> 5);
+  constexpr int W = kScoreWord<T, V>;
+  __shared__ __align__(16) float spread[kRouteWarps][32 * V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long t = blockIdx.x * (long long)kRouteWarps + warp;
   if (t >= tokens) return;
+  Pack<T, V, W> x;
+  if (!kNormalize) load_scores<T, V>(x, logits + t * stride, lane * W, 32 * W, experts, words);
   int mine = -1;
   float g = 0.f, w = 0.f;
   if (lane < top_k) {
     mine = chosen[t * top_k + lane];
-    if (mine >= 0 && mine < experts) {
-      g = grad[t * top_k + lane];
-      w = weights[t * top_k + lane];
-    } else {
-      mine = -1;
-    }
+    g = grad[t * top_k + lane];
+    w = weights[t * top_k + lane];
   }
+  if (mine < 0 || mine >= experts) {
+    mine = -1 - lane;
+    g = w = 0.f;
+  }
+  float* own = spread[warp];
+#pragma unroll
+  for (int v = 0; v < V; ++v) own[v * 32 + lane] = 0.f;
   const float inner = warp_sum(g * w);
-  float p[V], d[V];
+  float value = kNormalize ? w * (g - inner) : g;
+  const unsigned same = __match_any_sync(0xffffffffu, mine);
+  if (__any_sync(0xffffffffu, same & (same - 1)))  // a choice that stands twice: the first takes their sum
+    for (int j = 1; j < top_k; ++j) {
+      const float other = __shfl_sync(0xffffffffu, value, j);
+      if (j > lane && (same >> j & 1)) value += other;
+    }
+  if (mine >= 0 && lane == __ffs(same) - 1) own[mine] = value;
+  __syncwarp();
+  float top = -INFINITY, sum = 0.f, p[V];
   if (!kNormalize) {
-    float top, sum;
-    load_scores<T, V>(logits + t * stride, experts, p);
-    row_softmax<V>(p, top, sum);
-    const float inv = sum > 0.f ? 1.f / sum : sum;  // a NaN stays
 #pragma unroll
-    for (int v = 0; v < V; ++v) p[v] = expf(p[v] - top) * inv;
+    for (int v = 0; v < V; ++v) top = fmaxf(top, x.get(v));
+    top = fmaxf(kLowest, warp_max(top));
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += p[v] = expf(x.get(v) - top);
+    sum = warp_sum(sum);
+    sum = sum > 0.f ? 1.f / sum : sum;  // a NaN stays
   }
-#pragma unroll
-  for (int v = 0; v < V; ++v) d[v] = kNormalize ? 0.f : -p[v] * inner;
-  for (int j = 0; j < top_k; ++j) {
-    const int e = __shfl_sync(0xffffffffu, mine, j);
-    const float gj = __shfl_sync(0xffffffffu, g, j), wj = __shfl_sync(0xffffffffu, w, j);
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (e == v * 32 + lane) d[v] += kNormalize ? wj * (gj - inner) : p[v] * gj;
-  }
+  Pack<T, V, W> o;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = v * 32 + lane;
-    if (e < experts) out[t * out_stride + e] = from_float<T>(d[v]);
+    const float s = own[(v / W * 32 + lane) * W + v % W];
+    o.set(v, kNormalize ? s : p[v] * sum * (s - inner));
   }
+  if (words) o.store(out + t * out_stride, lane * W, 32 * W, experts);
+  else o.store_elements(out + t * out_stride, lane * W, 32 * W, experts);
 }
 
 // ---- order of the slots by expert ---------------------------------------------------
@@ -497,15 +525,20 @@ struct Count {
   static constexpr int value = N;
 };
 
-// f(V constant) with 32 * V >= experts.
-template <typename F>
-void with_scores(int experts, F&& f) {
-  if (experts <= 32) f(Count<1>());
-  else if (experts <= 64) f(Count<2>());
-  else if (experts <= 128) f(Count<4>());
-  else if (experts <= 256) f(Count<8>());
-  else if (experts <= 512) f(Count<16>());
-  else f(Count<32>());
+// Calls f(V, words): 32 * V >= experts, and whether every row allows the words
+// (fits(bytes): they begin at multiples of so many).
+template <typename T, typename Fits, typename F>
+void with_scores(int experts, Fits&& fits, F&& f) {
+  auto call = [&](auto v) {
+    constexpr int W = kScoreWord<T, decltype(v)::value>;
+    f(v, experts % W == 0 && fits(W * int(sizeof(T))));
+  };
+  if (experts <= 32) call(Count<1>());
+  else if (experts <= 64) call(Count<2>());
+  else if (experts <= 128) call(Count<4>());
+  else if (experts <= 256) call(Count<8>());
+  else if (experts <= 512) call(Count<16>());
+  else call(Count<32>());
 }
 
 int tail_blocks(bool zero_tail, long long rows) {
@@ -517,11 +550,13 @@ int tail_blocks(bool zero_tail, long long rows) {
 void route_launch(int dtype, RowsIn logits, int tokens, int experts, int top_k, bool normalize, float* weights, int* chosen,
                   cudaStream_t stream) {
   if (tokens == 0) return;
+  const int size = dtype_size(dtype);
+  auto fits = [&](int bytes) { return rows_aligned(logits.ptr, logits.stride, size, bytes); };
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    with_scores(experts, [&](auto v) {
+    with_scores<T>(experts, fits, [&](auto v, bool words) {
       route_tokens<T, decltype(v)::value><<<ceil_div(tokens, kRouteWarps), kRouteWarps * 32, 0, stream>>>(
-          static_cast<const T*>(logits.ptr), logits.stride, tokens, experts, top_k, normalize, weights, chosen);
+          static_cast<const T*>(logits.ptr), logits.stride, words, tokens, experts, top_k, normalize, weights, chosen);
     });
   });
   PSB_LAUNCH_CHECK();
@@ -530,13 +565,17 @@ void route_launch(int dtype, RowsIn logits, int tokens, int experts, int top_k, 
 void route_grad_launch(int dtype, const float* grad_weights, RowsIn logits, const float* weights, const int* chosen, int tokens,
                        int experts, int top_k, bool normalize, RowsOut grad_logits, cudaStream_t stream) {
   if (tokens == 0) return;
+  const int size = dtype_size(dtype);
+  auto fits = [&](int bytes) {
+    return rows_aligned(logits.ptr, logits.stride, size, bytes) && rows_aligned(grad_logits.ptr, grad_logits.stride, size, bytes);
+  };
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    with_scores(experts, [&](auto v) {
+    with_scores<T>(experts, fits, [&](auto v, bool words) {
       constexpr int V = decltype(v)::value;
       auto kernel = normalize ? route_grad_tokens<T, V, true> : route_grad_tokens<T, V, false>;
       kernel<<<ceil_div(tokens, kRouteWarps), kRouteWarps * 32, 0, stream>>>(
-          grad_weights, static_cast<const T*>(logits.ptr), logits.stride, weights, chosen, tokens, experts, top_k,
+          grad_weights, static_cast<const T*>(logits.ptr), logits.stride, words, weights, chosen, tokens, experts, top_k,
           static_cast<T*>(grad_logits.ptr), grad_logits.stride);
     });
   });

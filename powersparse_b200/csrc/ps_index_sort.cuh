@@ -29,7 +29,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxBits = 10, kMaxDigits = 1 << kMaxBits;  // one thread a digit
 constexpr int kKeep = 8;
-constexpr int kSortBlocks = 8;     // the largest cluster that needs no opt-in
+constexpr int kSortBlocks = 16;    // the largest cluster there is (above 8 it needs an opt-in)
 
 struct Strip {
   long long begin, end;
@@ -211,7 +211,7 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
 
 // Blocks of the cluster for n indices: one while each warp's strip is short, more as
 // the strips grow.
-inline int sort_blocks(long long n) { return n <= 2048 ? 1 : n <= 8192 ? 4 : kSortBlocks; }
+inline int sort_blocks(long long n) { return n <= 2048 ? 1 : n <= 8192 ? 4 : n <= 16384 ? 8 : kSortBlocks; }
 
 // A kernel launched with launch_after may start while the one before it still runs; it
 // waits here before it touches what that one writes, and reads that with plain loads
@@ -244,6 +244,7 @@ void launch_clusters(int blocks, long long clusters, int digits, cudaStream_t st
   const unsigned long long bit = device < 64 ? 1ULL << device : 0;
   if (!(prepared.load(std::memory_order_relaxed) & bit)) {
     PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sort_smem(kMaxDigits))));
+    PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     prepared.fetch_or(bit, std::memory_order_relaxed);
   }
   if (clusters * blocks > 0x7fffffffLL) throw std::invalid_argument("too many rows for one launch");

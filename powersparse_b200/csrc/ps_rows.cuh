@@ -46,6 +46,7 @@ struct Pack {
   static constexpr int kPart = kWordBytes < 16 ? kWordBytes : 16;
   static constexpr int kParts = kWordBytes / kPart;
   using Part = Word<kPart>;
+  using Element = Word<int(sizeof(T))>;
   union {
     Part w[N / W][kParts];
     unsigned char bytes[N * sizeof(T)];
@@ -73,6 +74,21 @@ struct Pack {
       if (c + i * step < width)
 #pragma unroll
         for (int k = 0; k < kParts; ++k) reinterpret_cast<Part*>(row + c + i * step)[k] = w[i][k];
+  }
+  // The same elements one at a time, for rows that do not allow the words.
+  __device__ __forceinline__ void load_elements(const T* row, int c, int step, int width) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int at = c + e / W * step + e % W;
+      if (at < width) reinterpret_cast<Element*>(bytes)[e] = __ldg(reinterpret_cast<const Element*>(row + at));
+    }
+  }
+  __device__ __forceinline__ void store_elements(T* row, int c, int step, int width) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int at = c + e / W * step + e % W;
+      if (at < width) reinterpret_cast<Element*>(row + at)[0] = reinterpret_cast<const Element*>(bytes)[e];
+    }
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll

@@ -153,7 +153,7 @@ def test_embedding_grad(dtype, out, width):
 
 
 @pytest.mark.parametrize("kind", ["any", "skewed", "one", "distinct", "sorted", "empty"])
-@pytest.mark.parametrize("n,rows", [(20000, 40000), (70001, 70001), (16384, 1025), (40000, 2_000_000), (9000, 512), (2049, 1023)])
+@pytest.mark.parametrize("n,rows", [(31, 9), (65, 5000), (2047, 300), (2048, 40000), (20000, 40000), (70001, 70001), (16384, 1025), (40000, 2_000_000), (9000, 512), (2049, 1023)])
 def test_embedding_grad_order_of_large_batches(kind, n, rows):
     g = gen(n + rows)
     if kind == "distinct" and n > rows:
@@ -175,13 +175,16 @@ def test_embedding_grad_of_a_million_tokens_and_many_passes():
     tokens = torch.tensor([3, 7, 3, 2**20, 7, 3, -1, 2**31 - 2, 2**31], device="cuda")
     out = torch.zeros(2**20 + 1, 8, device="cuda")
     lib = psb.load_library()
-    ws = torch.empty(lib.ps_embedding_grad_workspace(9, rows, 8), dtype=torch.uint8, device="cuda")
-    grad = randn(g, 9, 8)
     s = torch.cuda.current_stream().cuda_stream
-    assert lib.ps_embedding_grad(grad.data_ptr(), 0, 8, tokens.data_ptr(), 1, 9, 1.0, -1, 1, out.data_ptr(), 0, 8, rows, 8,
-                                 ws.data_ptr(), ws.numel(), s) == psb.PS_OK
-    want, slack = grad64(grad, tokens, 2**20 + 1, 1.0)
-    check(out, want, slack)
+    for times in (1, 1000):
+        many = tokens.repeat(times)
+        out.zero_()
+        ws = torch.empty(lib.ps_embedding_grad_workspace(9 * times, rows, 8) + 1, dtype=torch.uint8, device="cuda")
+        grad = randn(g, 9 * times, 8)
+        assert lib.ps_embedding_grad(grad.data_ptr(), 0, 8, many.data_ptr(), 1, 9 * times, 1.0, -1, 1, out.data_ptr(), 0, 8, rows, 8,
+                                     ws.data_ptr(), ws.numel(), s) == psb.PS_OK
+        want, slack = grad64(grad, many, 2**20 + 1, 1.0)
+        check(out, want, slack)
 
 
 def test_embedding_grad_padding_accumulate_and_no_tokens():
