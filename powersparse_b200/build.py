@@ -108,7 +108,7 @@ def build_rows_module(force: bool = False) -> str:
                                                     os.path.join(os.path.dirname(CUDA_LIBDIR), "include")]
         libs = os.path.join(os.path.dirname(torch.__file__), "lib")
         _run([HOSTCXX, "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-              *("-I" + i for i in includes), "-o", ROWS_MODULE, src, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu",
+              *("-I" + i for i in includes), "-o", ROWS_MODULE, src, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
               "-lc10_cuda", "-lc10"])
     return ROWS_MODULE
 

@@ -19,19 +19,19 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kRowUnroll = 4;
 
-template <typename T, int N, int W>
+template <typename T, int N, int W, int S>
 __global__ void __launch_bounds__(kRowThreads) embedding_rows(const T* __restrict__ table, long long table_stride, long long rows,
                                                               const void* __restrict__ tokens, bool wide, long long n, int width,
                                                               float scale, T* __restrict__ out, long long out_stride,
                                                               int lanes_log2) {
-  const int lanes = 1 << lanes_log2, step = lanes * W;
+  const int lanes = 1 << lanes_log2, step = word_step<W, S>(lanes);
   const long long i = blockIdx.x * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   if (i >= n) return;
   const long long token = index_at(tokens, wide, i);
   const bool inside = token >= 0 && token < rows;
   const T* src = table + (inside ? token : 0) * table_stride;
   T* dst = out + i * out_stride;
-  for (int c = (threadIdx.x & (lanes - 1)) * W; c < width; c += lanes * N * kRowUnroll) {
+  for (int c = first_column<N, W, S>(threadIdx.x & (lanes - 1)); c < width; c += lanes * N * kRowUnroll) {
     Pack<T, N, W> v[kRowUnroll];
 #pragma unroll
     for (int u = 0; u < kRowUnroll; ++u) {
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
 }
 
 // ---- gradient: sums of the sorted rows ----------------------------------------------
-// A block takes `chunk` consecutive sorted positions and kSumThreads * N columns, and
+// A block takes `chunk` consecutive sorted positions and N columns a thread, and
 // adds the gradient rows run by run in 32-bit registers.  A run inside the chunk goes
 // to its row; what belongs to a run that crosses a border goes to the chunk's two
 // partial rows: [0] for the run that began before the chunk, [1] for one that goes on
@@ -158,15 +158,15 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
   const int count = int(min((long long)chunk, n - first));
   let_next_start();
   wait_for_previous();
-  for (int i = threadIdx.x; i < count + 2; i += kSumThreads) {
+  for (int i = threadIdx.x; i < count + 2; i += blockDim.x) {
     const long long p = first + i - 1;
     const Item item = p >= 0 && p < n ? items[p] : Item{kNone, 0};
     key[i] = item.token;
     if (i >= 1 && i <= count) at[i - 1] = item.place;
   }
   __syncthreads();
-  constexpr int kStep = kSumThreads * W;
-  const int c = blockIdx.y * kSumThreads * N + threadIdx.x * W;
+  constexpr int step = 32 * W;
+  const int c = first_column<N, W, 32>(blockIdx.y * blockDim.x + threadIdx.x);
   if (c >= width) return;
   float acc[N];
 #pragma unroll
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
     Pack<T, N, W> v[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (i + u < count && key[i + u + 1] < rows) v[u].load(grad + (long long)at[i + u] * grad_stride, c, kStep, width);
+      if (i + u < count && key[i + u + 1] < rows) v[u].load(grad + (long long)at[i + u] * grad_stride, c, step, width);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       if (i + u >= count) break;
@@ -187,12 +187,12 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
       if (key[i + u + 2] == k && i + u + 1 < count) continue;
       const bool after = key[i + u + 2] == k;
       if (!before && !after) {
-        write_sum<O, N, W>(out + (long long)k * out_stride, c, kStep, width, acc, scale, accumulate);
+        write_sum<O, N, W>(out + (long long)k * out_stride, c, step, width, acc, scale, accumulate);
       } else {
         Pack<float, N, W> sum;
 #pragma unroll
         for (int e = 0; e < N; ++e) sum.set(e, acc[e]);
-        sum.store(partial + (blockIdx.x * 2LL + (before ? 0 : 1)) * width, c, kStep, width);
+        sum.store(partial + (blockIdx.x * 2LL + (before ? 0 : 1)) * width, c, step, width);
       }
       before = false;
 #pragma unroll
@@ -202,46 +202,81 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
 }
 
 // The runs that cross a border, by the list of their tokens and the chunks in which
-// they begin: their partial rows, added in order by each of the block's warps (every
-// kJoinWarps-th chunk) and then over the warps.
+// they begin: a warp for one of them and the 32 * N columns of blockIdx.y.  A run of at
+// most kShortRun chunks, as nearly all are, is added up by its warp alone; the block's
+// warps join in a longer one (every kJoinWarps-th chunk each, then over the warps).
 constexpr int kJoinWarps = 8;
+constexpr int kShortRun = 4;
 
 template <typename O, int N, int W>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, long long n, int width, float scale,
                                                              bool accumulate, O* __restrict__ out, long long out_stride, int chunk,
                                                              const float* partial, const Item* joins, const int* join_count,
-                                                             long long most) {
+                                                             int most) {
+  constexpr int kUnroll = 4;
   __shared__ float sums[kJoinWarps][32 * N];
+  __shared__ bool is_long[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int slabs = ceil_div(width, 32 * N);
+  const int c = blockIdx.y * 32 * N + lane * W;
   wait_for_previous();
-  for (long long i = blockIdx.x; i < most; i += gridDim.x) {
-    const Item join = joins[i / slabs];  // read beside the count, not after it: there is room for `most`
-    if (i >= (long long)*join_count * slabs) return;
-    const int c = int(i % slabs) * 32 * N + lane * W;
+  // Adds the shares of the chunks own + first, own + first + stride, ... (kUnroll of them at
+  // most) of the run that begins in chunk `own`; whether the last of them belongs to it.
+  auto add = [&](float (&acc)[N], Item join, long long first, int stride) {
     const long long own = join.place;
+    Pack<float, N, W> v[kUnroll];
+    bool on[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const long long j = own + first + u * stride;
+      const bool inside = j * chunk < n;
+      v[u].zero();
+      if (inside) v[u].load_rw(partial + (j * 2 + (j == own ? 1 : 0)) * width, c, 32 * W, width);
+      on[u] = j == own || (inside && items[j * chunk].token == join.token);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += on[u] ? v[u].get(e) : 0.f;
+    return on[kUnroll - 1];
+  };
+  for (int first = blockIdx.x * kJoinWarps; first < most; first += gridDim.x * kJoinWarps) {
+    const int work = *join_count;
+    if (first >= work) return;
+    const Item join = joins[min(first + warp, most - 1)];  // read beside the count, not after it: there is room for `most`
+    bool longer = false;
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
-    for (long long j = own + warp; j * chunk < n && (j == own || items[j * chunk].token == join.token); j += kJoinWarps) {
-      if (c < width) {
-        Pack<float, N, W> v;
-        v.zero();
-        v.load_rw(partial + (j * 2 + (j == own ? 1 : 0)) * width, c, 32 * W, width);
-#pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += v.get(e);
+    if (first + warp < work) {
+      static_assert(kUnroll == kShortRun);
+      const long long next = (long long)join.place + kShortRun;
+      longer = next * chunk < n && items[next * chunk].token == join.token;
+      if (!longer) {
+        add(acc, join, 0, 1);
+        if (c < width) write_sum<O, N, W>(out + (long long)join.token * out_stride, c, 32 * W, width, acc, scale, accumulate);
       }
     }
-#pragma unroll
-    for (int e = 0; e < N; ++e) sums[warp][e * 32 + lane] = acc[e];
+    if (!__syncthreads_or(longer)) continue;
+    if (lane == 0) is_long[warp] = longer;
     __syncthreads();
-    if (warp == 0 && c < width) {
-      for (int w = 1; w < kJoinWarps; ++w)
+    for (int k = 0; k < kJoinWarps; ++k) {
+      if (!is_long[k]) continue;
+      const Item other = joins[first + k];
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += sums[w][e * 32 + lane];
-      write_sum<O, N, W>(out + (long long)join.token * out_stride, c, 32 * W, width, acc, scale, accumulate);
+      for (int e = 0; e < N; ++e) acc[e] = 0.f;
+      for (long long j = warp; add(acc, other, j, kJoinWarps); j += kJoinWarps * kUnroll) {
+      }
+#pragma unroll
+      for (int e = 0; e < N; ++e) sums[warp][e * 32 + lane] = acc[e];
+      __syncthreads();
+      if (warp == 0 && c < width) {
+        for (int w = 1; w < kJoinWarps; ++w)
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[e] += sums[w][e * 32 + lane];
+        write_sum<O, N, W>(out + (long long)other.token * out_stride, c, 32 * W, width, acc, scale, accumulate);
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -269,7 +304,7 @@ __device__ __forceinline__ void few_tokens(const void* tokens, bool wide, int n,
   }
 }
 
-template <typename T, typename O, int N, int W>
+template <typename T, typename O, int N, int W, int S>
 __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ grad, long long grad_stride,
                                                        const void* __restrict__ tokens, bool wide, int n, long long rows,
                                                        long long padding, int width, float scale, bool accumulate,
@@ -331,9 +366,9 @@ __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ gra
 
   constexpr int kUnroll = 4;
   const int lanes = total > kLongRun ? 32 : 1 << lanes_log2, groups = kFewThreads / lanes;  // threads a row, rows at a time
-  const int group = threadIdx.x / lanes, step = lanes * W;
+  const int group = threadIdx.x / lanes, step = word_step<W, S>(lanes);
   for (int slab = 0; slab < width; slab += lanes * N) {
-    const int c = slab + (threadIdx.x & (lanes - 1)) * W;
+    const int c = slab + first_column<N, W, S>(threadIdx.x & (lanes - 1));
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
@@ -392,10 +427,10 @@ void embedding_launch(int dtype, RowsIn table, long long rows, int width, Indice
       return rows_aligned(table.ptr, table.stride, size, bytes) && rows_aligned(out.ptr, out.stride, size, bytes);
     };
     with_shape<T>(width, fits, [&](auto shape) {
-      constexpr int N = decltype(shape)::N, W = decltype(shape)::W;
-      const int lanes_log2 = row_lanes(ceil_div(width, N), kRowUnroll, 0);
+      constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;
+      const int lanes_log2 = row_lanes(width, N * kRowUnroll, 1, decltype(shape)::kLeastLanesLog2, tokens.count);
       const unsigned blocks = grid_x(ceil_div_ll(tokens.count, kRowThreads >> lanes_log2));
-      embedding_rows<T, N, W><<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(table.ptr), table.stride, rows, tokens.ptr,
+      embedding_rows<T, N, W, S><<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(table.ptr), table.stride, rows, tokens.ptr,
                                                                   tokens.wide, tokens.count, width, scale,
                                                                   static_cast<T*>(out.ptr), out.stride, lanes_log2);
     });
@@ -433,25 +468,26 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
       return rows_aligned(grad.ptr, grad.stride, in_size, bytes) && rows_aligned(out.ptr, out.stride, out_size, bytes);
     };
     with_shape<T>(width, fits, [&](auto shape) {
-      constexpr int N = decltype(shape)::N, W = decltype(shape)::W;
+      constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;
       O* dst = static_cast<O*>(out.ptr);
       if (few) {
         const int clear_rows = int(std::min<long long>(kClearRows, std::max<long long>(1, kClearBytes / row_bytes)));
         const long long blocks = n + (accumulate ? 0 : ceil_div_ll(rows, clear_rows));  // n and blocks are not both 0
-        sum_few<T, O, N, W><<<grid_x(blocks), kFewThreads, 0, stream>>>(
+        sum_few<T, O, N, W, S><<<grid_x(blocks), kFewThreads, 0, stream>>>(
             static_cast<const T*>(grad.ptr), grad.stride, tokens.ptr, tokens.wide, int(n), rows, padding, width, scale, accumulate,
-            dst, out.stride, clear_rows, row_lanes(ceil_div(width, N), 1, 2));
+            dst, out.stride, clear_rows, row_lanes(width, N, 1, std::max(2, decltype(shape)::kLeastLanesLog2), n));
         PSB_LAUNCH_CHECK();
         return;
       }
       const unsigned chunks = grid_x(ceil_div_ll(n, chunk));
-      const dim3 sums(chunks, unsigned(ceil_div(width, kSumThreads * N)));
-      launch_after(sum_runs<T, O, N, W>, sums, kSumThreads, stream, static_cast<const T*>(grad.ptr), grad.stride, items, n,
+      // As few blocks a row as kSumThreads allows, and no more warps in them than the row fills.
+      const int slabs = ceil_div(width, kSumThreads * N), threads = ceil_div(ceil_div(width, slabs * N), 32) * 32;
+      launch_after(sum_runs<T, O, N, W>, dim3(chunks, unsigned(slabs)), threads, stream, static_cast<const T*>(grad.ptr), grad.stride, items, n,
                    uint32_t(rows), width, scale, accumulate, dst, out.stride, chunk, partial);
       if (chunks == 1) return;
-      const long long most = (long long)(chunks - 1) * ceil_div(width, 32 * N);
-      launch_after(join_runs<O, N, W>, unsigned(std::min<long long>(most, 8LL * device_sms())), kJoinWarps * 32, stream, items, n,
-                   width, scale, accumulate, dst, out.stride, chunk, partial, joins, join_count, most);
+      const dim3 joining(unsigned(std::min(ceil_div(int(chunks) - 1, kJoinWarps), 8 * device_sms())), unsigned(ceil_div(width, 32 * N)));
+      launch_after(join_runs<O, N, W>, joining, kJoinWarps * 32, stream, items, n, width, scale, accumulate, dst, out.stride, chunk,
+                   partial, joins, join_count, int(chunks) - 1);
     });
   };
   with_type(grad_dtype, [&](auto t) {

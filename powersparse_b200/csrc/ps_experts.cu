@@ -409,16 +409,16 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsign
     copy_row<B>(x + t * x_bytes, position + t * top_k, top_k, blanks.rows, words, out, out_bytes, 1 << lanes_log2);
 }
 
-template <typename T, int N, int W, bool kWeighted>
+template <typename T, int N, int W, int S, bool kWeighted>
 __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict__ y, long long y_stride, long long rows,
                                                             const int* __restrict__ position, const float* __restrict__ weights,
                                                             const T* add, long long add_stride, int tokens, int top_k, int width,
                                                             T* out, long long out_stride, int lanes_log2) {
   constexpr int kSlots = 4;  // rows in flight
-  const int lanes = 1 << lanes_log2, step = lanes * W;
+  const int lanes = 1 << lanes_log2, step = word_step<W, S>(lanes);
   const long long t = blockIdx.x * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   if (t >= tokens) return;
-  for (int c = (threadIdx.x & (lanes - 1)) * W; c < width; c += lanes * N) {
+  for (int c = first_column<N, W, S>(threadIdx.x & (lanes - 1)); c < width; c += lanes * N) {
     float acc[N];
     Pack<T, N, W> o;
     o.zero();
@@ -451,8 +451,8 @@ __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict_
   }
 }
 
-template <typename T, int N, int W>
-__global__ void __launch_bounds__(kRowThreads) combine_grad_rows(const T* __restrict__ grad, long long grad_stride, const T* y,
+template <typename T, int N, int W, int S>
+__global__ void __launch_bounds__(kRowThreads, 3) combine_grad_rows(const T* __restrict__ grad, long long grad_stride, const T* y,
                                                                  long long y_stride, const int* __restrict__ position,
                                                                  Blanks blanks, const float* __restrict__ weights, int tokens,
                                                                  int top_k, int width, T* grad_y, long long grad_y_stride,
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_rows(const T* __rest
                                            grad_y_stride * (long long)sizeof(T));
   const long long rows = blanks.rows;
   __shared__ float parts[kRowThreads / 32][kSlots];
-  const int lanes = 1 << lanes_log2, step = lanes * W;  // 32 lanes at least
+  const int lanes = 1 << lanes_log2, step = word_step<W, S>(lanes);  // 32 lanes at least
   const long long t = (blockIdx.x - blanks.blocks()) * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   const bool live = t < tokens;  // the whole warp; the others take part in the block's barriers
   for (int j0 = 0; j0 < top_k; j0 += kSlots) {
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_grad_rows(const T* __rest
       dot[s] = 0.f;
     }
     if (live) {
-      for (int c = (threadIdx.x & (lanes - 1)) * W; c < width; c += lanes * N) {
+      for (int c = first_column<N, W, S>(threadIdx.x & (lanes - 1)); c < width; c += lanes * N) {
         Pack<T, N, W> g, v[kSlots];
         g.zero();
         g.load(grad + t * grad_stride, c, step, width);
@@ -600,7 +600,7 @@ void dispatch_launch(int dtype, RowsIn x, Indices chosen, int tokens, int top_k,
     constexpr int B = decltype(bytes)::value;
     const auto* src = static_cast<const unsigned char*>(x.ptr);
     auto* dst = static_cast<unsigned char*>(out.ptr);
-    const int words = int(row_bytes / B), lanes_log2 = few ? row_lanes(words, 1, 5) : row_lanes(words, kRowUnroll, 0);
+    const int words = int(row_bytes / B), lanes_log2 = few ? row_lanes(words, 1, 1, 5, tokens) : row_lanes(words, kRowUnroll, 1, 0, tokens);
     const long long blocks = blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2);
     if (few)
       dispatch_few<B><<<grid_x(std::max(1LL, blocks)), kRowThreads, 0, stream>>>(
@@ -630,10 +630,10 @@ void combine_launch(int dtype, RowsIn y, long long rows, const int* position, co
              (!add.ptr || rows_aligned(add.ptr, add.stride, size, bytes));
     };
     with_shape<T>(width, fits, [&](auto shape) {
-      constexpr int N = decltype(shape)::N, W = decltype(shape)::W;
-      const int lanes_log2 = row_lanes(ceil_div(width, N), 2, 0);
+      constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;
+      const int lanes_log2 = row_lanes(width, N, 2, decltype(shape)::kLeastLanesLog2, tokens);
       const unsigned blocks = grid_x(ceil_div_ll(tokens, kRowThreads >> lanes_log2));
-      auto kernel = weights ? combine_rows<T, N, W, true> : combine_rows<T, N, W, false>;
+      auto kernel = weights ? combine_rows<T, N, W, S, true> : combine_rows<T, N, W, S, false>;
       kernel<<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(y.ptr), y.stride, rows, position, weights,
                                                  static_cast<const T*>(add.ptr), add.stride, tokens, top_k, width,
                                                  static_cast<T*>(out.ptr), out.stride, lanes_log2);
@@ -654,10 +654,10 @@ void combine_grad_launch(int dtype, RowsIn grad, RowsIn y, long long rows, const
              rows_aligned(grad_y.ptr, grad_y.stride, size, bytes);
     };
     with_shape<T>(width, fits, [&](auto shape) {
-      constexpr int N = decltype(shape)::N, W = decltype(shape)::W;
-      const int lanes_log2 = row_lanes(ceil_div(width, N), 8, 5);
+      constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;
+      const int lanes_log2 = row_lanes(width, N, 8, 5, tokens);
       const unsigned blocks = grid_x(blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2));
-      combine_grad_rows<T, N, W><<<blocks, kRowThreads, 0, stream>>>(
+      combine_grad_rows<T, N, W, S><<<blocks, kRowThreads, 0, stream>>>(
           static_cast<const T*>(grad.ptr), grad.stride, static_cast<const T*>(y.ptr), y.stride, position, blanks, weights, tokens,
           top_k, width, static_cast<T*>(grad_y.ptr), grad_y.stride, grad_weights, lanes_log2);
     });

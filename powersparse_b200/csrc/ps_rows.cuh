@@ -117,21 +117,42 @@ inline bool rows_aligned(const void* ptr, long long stride, int size, int bytes)
   return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && (stride * size) % bytes == 0;
 }
 
-// Elements a thread holds (N) and elements of a word (W).
-template <int N_, int W_>
+// How the threads of a row share it: N elements a thread and turn, in words of W.  S = 32:
+// a warp takes 32 * N columns, its words 32 apart, so that the distances are constants;
+// S = 0: for rows that less than a warp shares, the words stand as far apart as there
+// are threads.
+template <int N_, int W_, int S_>
 struct Shape {
-  static constexpr int N = N_, W = W_;
+  static constexpr int N = N_, W = W_, S = S_;
+  // For 32 threads at least where the words are apart by a constant.
+  static constexpr int kLeastLanesLog2 = S && W != N ? 5 : 0;
 };
+
+// First column of thread t of the row's 2^k lanes in its first turn, and the distance of its words.
+template <int N, int W, int S>
+__device__ __forceinline__ int first_column(int t) {
+  return S ? t / 32 * 32 * N + t % 32 * W : t * W;
+}
+template <int W, int S>
+__device__ __forceinline__ int word_step(int lanes) {
+  return S ? S * W : lanes * W;
+}
 
 // Calls f(Shape) for rows of `width` elements of type T: words of 16 bytes where
 // fits(16) says that every operand's rows allow them, of 4 bytes where fits(4) does,
-// else single elements.  fits need not look at the width.
+// else single elements, four words a thread.  fits need not look at the width.
 template <typename T, typename Fits, typename F>
 void with_shape(int width, Fits&& fits, F&& f) {
   constexpr int kSize = int(sizeof(T)), kN = 16 / kSize, kHalf = 4 / kSize;
-  if (width % kN == 0 && fits(16)) f(Shape<kN, kN>());
-  else if (kHalf > 1 && width % kHalf == 0 && fits(4)) f(Shape<kN, kHalf>());
-  else f(Shape<kN, 1>());
+  if (width % kN == 0 && fits(16)) {
+    f(Shape<kN, kN, 32>());
+  } else if (kHalf > 1 && width % kHalf == 0 && fits(4)) {
+    if (width > 16 * kN) f(Shape<kN, kHalf, 32>());
+    else f(Shape<kN, kHalf, 0>());
+  } else {
+    if (width > 64) f(Shape<4, 1, 32>());
+    else f(Shape<4, 1, 0>());
+  }
 }
 
 // log2 of the smallest power of two >= v.
@@ -141,9 +162,15 @@ inline int log2_up(long long v) {
   return b;
 }
 
-// log2 of the threads that share a row of `words` words, `each` of them a thread.
-inline int row_lanes(int words, int each, int least_log2) {
-  return std::min(8, std::max(least_log2, log2_up(ceil_div(words, each))));
+// log2 of the threads that share a row of `width` elements, `n` of them a thread and
+// turn: as many as give a row `turns` turns; fewer where the last turn would leave more
+// than a fifth of the work empty and the `rows` fill the GPU's threads twice over.
+inline int row_lanes(int width, int n, int turns, int least_log2, long long rows) {
+  int lanes = std::min(8, std::max(least_log2, log2_up(ceil_div(ceil_div(width, n), turns))));
+  while (lanes > std::max(5, least_log2) && rows << lanes >= 4096LL * device_sms() &&
+         (long long)ceil_div(width, n << lanes) * (n << lanes) * 4 > 5LL * width)
+    --lanes;
+  return lanes;
 }
 
 inline unsigned grid_x(long long blocks) {

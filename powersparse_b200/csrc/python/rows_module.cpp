@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -129,8 +130,13 @@ Matrix matrix_like(PyObject* o, const char* name, c10::Device device, at::Scalar
   return m;
 }
 
+// torch.empty without the dispatcher, which took longer than the allocation.
+at::Tensor new_tensor(at::IntArrayRef shape, at::ScalarType type, c10::Device device) {
+  return at::detail::empty_cuda(shape, type, device, std::nullopt);
+}
+
 Matrix new_matrix(int64_t rows, int64_t width, const at::Tensor& like, at::ScalarType type) {
-  at::Tensor t = at::empty({rows, width}, like.options().dtype(type).requires_grad(false));
+  at::Tensor t = new_tensor({rows, width}, type, like.device());
   void* p = t.data_ptr();
   return {std::move(t), rows, width, width, type_of(type), p};
 }
@@ -293,7 +299,7 @@ PyObject* embedding_grad(PyObject* const* a) {  // grad, tokens, rows, scale, pa
   {
     WithoutGil nogil;
     if (fresh) out = new_matrix(rows, grad.width, grad.t, type);
-    const at::Tensor workspace = at::empty({need}, given.options().dtype(at::kByte).requires_grad(false));
+    const at::Tensor workspace = new_tensor({need}, at::kByte, device);
     check(api.embedding_grad(grad.ptr, grad.type, grad.stride, tokens.data_ptr(), index_type, n, scale, padding, accumulate, out.ptr,
                              out.type, out.stride, rows, int(grad.width), workspace.data_ptr(), need, place.handle()));
   }
@@ -311,9 +317,8 @@ PyObject* route(PyObject* const* a) {  // logits, top_k, normalize, stream
   at::Tensor weights, chosen;
   {
     WithoutGil nogil;
-    const auto options = logits.t.options().requires_grad(false);
-    weights = at::empty({logits.rows, top_k}, options.dtype(at::kFloat));
-    chosen = at::empty({logits.rows, top_k}, options.dtype(at::kInt));
+    weights = new_tensor({logits.rows, top_k}, at::kFloat, logits.t.device());
+    chosen = new_tensor({logits.rows, top_k}, at::kInt, logits.t.device());
     check(api.route(logits.ptr, logits.type, logits.stride, int(logits.rows), int(logits.width), int(top_k), normalize,
                     static_cast<float*>(weights.data_ptr()), static_cast<int*>(chosen.data_ptr()), place.handle()));
   }
@@ -373,10 +378,9 @@ PyObject* dispatch(PyObject* const* a) {  // x, chosen, num_experts, align, out,
   {
     WithoutGil nogil;
     if (fresh) out = new_matrix(need, x.width, x.t, x.t.scalar_type());
-    const auto options = x.t.options().dtype(at::kInt).requires_grad(false);
-    position = at::empty({x.rows, top_k}, options);
-    offsets = at::empty({experts + 1}, options);
-    counts = at::empty({experts}, options);
+    position = new_tensor({x.rows, top_k}, at::kInt, device);
+    offsets = new_tensor({experts + 1}, at::kInt, device);
+    counts = new_tensor({experts}, at::kInt, device);
     check(api.dispatch(x.ptr, x.type, x.stride, chosen.data_ptr(), index_type, int(x.rows), int(top_k), int(experts), int(align),
                        int(x.width), out.ptr, out.stride, out.rows, fresh, static_cast<int*>(position.data_ptr()),
                        static_cast<int*>(offsets.data_ptr()), static_cast<int*>(counts.data_ptr()), place.handle()));
@@ -435,7 +439,7 @@ PyObject* combine_grad(PyObject* const* a) {  // grad, y, position, offsets, cou
   {
     WithoutGil nogil;
     if (fresh) out = new_matrix(y.rows, y.width, y.t, y.t.scalar_type());
-    grad_weights = at::empty({plan.tokens, plan.top_k}, y.t.options().dtype(at::kFloat).requires_grad(false));
+    grad_weights = new_tensor({plan.tokens, plan.top_k}, at::kFloat, device);
     check(api.combine_grad(grad.ptr, y.type, grad.stride, y.ptr, y.stride, y.rows, static_cast<const int*>(plan.position.data_ptr()),
                            static_cast<const int*>(plan.offsets.data_ptr()), static_cast<const int*>(plan.counts.data_ptr()),
                            int(plan.experts), static_cast<const float*>(weights.data_ptr()), int(plan.tokens), int(plan.top_k),
