@@ -19,6 +19,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -62,10 +63,12 @@ def build_cuda(force: bool = False) -> str:
     deps = srcs + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh")) + \
         [os.path.join(INCLUDE, "powersparse_b200.h")]
     os.makedirs(LIB, exist_ok=True)
-    for target, flags in ((CUDA_LIB, []), (CHECKED_LIB, ["-DPSB_BOUNDS_CHECK=1"])):
-        if force or _stale(target, deps):
-            _run([NVCC, "-std=c++17", "-O3", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC", "-shared", *flags,
-                  "-ccbin", HOSTCXX, "-I" + INCLUDE, "-o", target, *srcs])
+    stale = [(target, flags) for target, flags in ((CUDA_LIB, []), (CHECKED_LIB, ["-DPSB_BOUNDS_CHECK=1"]))
+             if force or _stale(target, deps)]
+    # The sources of a library, and the two libraries, are compiled side by side.
+    with ThreadPoolExecutor(2) as pool:
+        list(pool.map(lambda job: _run([NVCC, "-std=c++17", "-O3", *ARCH, "-lineinfo", "--threads", "0", "-Xcompiler", "-fPIC",
+                                        "-shared", *job[1], "-ccbin", HOSTCXX, "-I" + INCLUDE, "-o", job[0], *srcs]), stale))
     return CUDA_LIB
 
 

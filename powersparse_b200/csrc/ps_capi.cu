@@ -312,7 +312,7 @@ int ps_embedding(const void* table, int dtype, long long rows, int width, long l
 
 long long ps_embedding_grad_workspace(long long n, long long rows, int width) {
   if (n < 0 || n > 0x7fffffffLL || rows < 1 || rows >= 0x7fffffffLL || width < 1 || width > (1 << 24)) return -1;
-  return (long long)psb::embedding_grad_workspace(n, width);
+  return (long long)psb::embedding_grad_workspace(n, rows, width);
 }
 
 int ps_embedding_grad(const void* grad, int grad_dtype, long long grad_stride, const void* tokens, int index_type, long long n,
@@ -326,7 +326,7 @@ int ps_embedding_grad(const void* grad, int grad_dtype, long long grad_stride, c
     require(rows >= 1 && rows < 0x7fffffffLL, what, "the table's rows must be in [1, 2^31 - 2]");
     require_rows(grad, grad_stride, n, width, in_size, what);
     require_rows(grad_table, table_stride, rows, width, out_size, what);
-    const long long need = (long long)psb::embedding_grad_workspace(n, width);
+    const long long need = (long long)psb::embedding_grad_workspace(n, rows, width);
     require(workspace_bytes >= need && (workspace != nullptr || need == 0), what,
             "the workspace is smaller than ps_embedding_grad_workspace says");
     require(reinterpret_cast<uintptr_t>(workspace) % 256 == 0, what, "the workspace must begin at a multiple of 256 bytes");

@@ -85,15 +85,41 @@ struct Clear {
   }
 };
 
+// The rows of a large gradient that the sort leaves to the kernels after it, cleared
+// beside their sums: rows [begin, end) that no token names, by blocks of whole warps.
+struct Rest {
+  unsigned char* ptr;
+  const unsigned char* touched;
+  long long begin, end, bytes, pitch;
+  static constexpr int kBytes = 1 << 16;  // of a block
+  __host__ __device__ long long block_rows() const { return bytes >= kBytes ? 1 : kBytes / bytes; }
+  __host__ long long blocks() const { return ceil_div_ll(end - begin, block_rows()); }
+  __device__ void run(long long block) const {
+    const long long first = begin + block * block_rows(), last = min(end, first + block_rows());
+    for (long long r = first + (threadIdx.x >> 5); r < last; r += blockDim.x >> 5)
+      if (!touched[r]) clear(ptr + r * pitch, bytes, threadIdx.x & 31, 32);
+  }
+};
+
 // The first cluster sorts the tokens; tokens outside [0, rows) and the padding token
 // get the key `rows` and come last.  The sorted items are in `a`.  Then it lists the
 // chunks of sorted items in which a run of one token begins that goes on in the next
-// chunk (join_count of them, in any order).  The other clusters clear the gradient
-// meanwhile: rows that no token names need it, and what the others cost is hidden,
-// since the sort leaves most of the GPU idle.
+// chunk, those of at most kShortRun chunks (at least two) and the longer ones apart, in any order.  The
+// other clusters clear the gradient meanwhile, or the first rows of a large one: rows
+// that no token names need it, and what the others cost is hidden, since the sort
+// leaves most of the GPU idle.  touched (null unless rows are left to the later
+// kernels): 1 for every token that occurs.
+constexpr int kShortRun = 4;
+
+struct Joins {
+  Item* shorter;  // token and chunk
+  Item* longer;
+  int* count;  // of the two
+};
+
 __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __restrict__ tokens, bool wide, long long n,
                                                                 long long rows, long long padding, int pass_bits, int passes,
-                                                                Item* a, Item* b, int chunk, Item* joins, int* join_count,
+                                                                Item* a, Item* b, int chunk, Joins joins, unsigned char* touched,
                                                                 Clear zeros) {
   extern __shared__ uint32_t smem[];
   namespace cg = cooperative_groups;
@@ -104,7 +130,9 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
   const int digits = 1 << pass_bits;
   const SortShared sh(smem, digits);
   const Strip strip = warp_strip(n, rank, blocks);
-  if (rank == 0 && threadIdx.x == 0) *join_count = 0;
+  if (rank == 0 && threadIdx.x < 2) joins.count[threadIdx.x] = 0;
+  if (touched)
+    for (long long v = rank * kSortThreads + threadIdx.x; v < rows; v += blocks * kSortThreads) touched[v] = 0;
   for (int pass = 0; pass < passes; ++pass) {
     const bool to_a = ((passes - 1 - pass) & 1) == 0;
     Item* out = to_a ? a : b;
@@ -118,12 +146,18 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
           return {uint32_t(t >= 0 && t < rows && t != padding ? t : rows), uint32_t(i)};
         },
         [&](Item e) { return int((e.token >> shift) & uint32_t(digits - 1)); }, [](uint32_t count) { return count; },
-        [](int, uint32_t, uint32_t) {}, [&](long long, Item e, uint32_t p) { out[p] = e; });
+        [](int, uint32_t, uint32_t) {},
+        [&](long long, Item e, uint32_t p) {
+          out[p] = e;
+          if (touched && pass == 0 && e.token < rows) touched[e.token] = 1;  // cleared before the barrier of the pass
+        });
   }
   for (long long c = rank * kSortThreads + threadIdx.x; (c + 1) * chunk < n; c += blocks * kSortThreads) {
     const uint32_t token = a[(c + 1) * chunk - 1].token;
-    if (token < rows && a[(c + 1) * chunk].token == token && (c == 0 || a[c * chunk - 1].token != token))
-      joins[atomicAdd(join_count, 1)] = {token, uint32_t(c)};
+    if (token < rows && a[(c + 1) * chunk].token == token && (c == 0 || a[c * chunk - 1].token != token)) {
+      const bool longer = (c + kShortRun) * chunk < n && a[(c + kShortRun) * chunk].token == token;
+      (longer ? joins.longer : joins.shorter)[atomicAdd(joins.count + longer, 1)] = {token, uint32_t(c)};
+    }
   }
 }
 
@@ -150,14 +184,15 @@ template <typename T, typename O, int N, int W>
 __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ grad, long long grad_stride,
                                                         const Item* items, long long n, uint32_t rows, int width, float scale, bool accumulate,
                                                         O* __restrict__ out, long long out_stride, int chunk,
-                                                        float* __restrict__ partial) {
+                                                        float* __restrict__ partial, int sum_blocks, int slabs, Rest rest) {
   constexpr int kUnroll = 8;
   constexpr uint32_t kNone = 0xffffffffu;
   __shared__ uint32_t key[kMaxChunk + 2], at[kMaxChunk];
-  const long long first = blockIdx.x * (long long)chunk;
-  const int count = int(min((long long)chunk, n - first));
   let_next_start();
   wait_for_previous();
+  if (int(blockIdx.x) >= sum_blocks) return rest.run(blockIdx.x - sum_blocks);
+  const long long block = blockIdx.x / slabs, first = block * chunk;
+  const int count = int(min((long long)chunk, n - first));
   for (int i = threadIdx.x; i < count + 2; i += blockDim.x) {
     const long long p = first + i - 1;
     const Item item = p >= 0 && p < n ? items[p] : Item{kNone, 0};
@@ -166,7 +201,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
   }
   __syncthreads();
   constexpr int step = 32 * W;
-  const int c = first_column<N, W, 32>(blockIdx.y * blockDim.x + threadIdx.x);
+  const int c = first_column<N, W, 32>(blockIdx.x % slabs * blockDim.x + threadIdx.x);
   if (c >= width) return;
   float acc[N];
 #pragma unroll
@@ -192,7 +227,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
         Pack<float, N, W> sum;
 #pragma unroll
         for (int e = 0; e < N; ++e) sum.set(e, acc[e]);
-        sum.store(partial + (blockIdx.x * 2LL + (before ? 0 : 1)) * width, c, step, width);
+        sum.store(partial + (block * 2 + (before ? 0 : 1)) * width, c, step, width);
       }
       before = false;
 #pragma unroll
@@ -201,27 +236,26 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
   }
 }
 
-// The runs that cross a border, by the list of their tokens and the chunks in which
-// they begin: a warp for one of them and the 32 * N columns of blockIdx.y.  A run of at
-// most kShortRun chunks, as nearly all are, is added up by its warp alone; the block's
-// warps join in a longer one (every kJoinWarps-th chunk each, then over the warps).
+// The runs that cross a border, 32 * N columns at a time.  Blocks first take the longer
+// ones, all their warps one run (every kJoinWarps-th chunk each, then over the warps);
+// the `short_blocks` behind them take a short one a warp.
 constexpr int kJoinWarps = 8;
-constexpr int kShortRun = 4;
 
 template <typename O, int N, int W>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, long long n, int width, float scale,
                                                              bool accumulate, O* __restrict__ out, long long out_stride, int chunk,
-                                                             const float* partial, const Item* joins, const int* join_count,
-                                                             int most) {
-  constexpr int kUnroll = 4;
+                                                             const float* partial, Joins joins, int chunks, int long_blocks,
+                                                             int short_blocks, int slabs, Rest rest) {
+  constexpr int kUnroll = kShortRun;
   __shared__ float sums[kJoinWarps][32 * N];
-  __shared__ bool is_long[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = blockIdx.y * 32 * N + lane * W;
   wait_for_previous();
+  if (int(blockIdx.x) >= (long_blocks + short_blocks) * slabs) return rest.run(blockIdx.x - (long_blocks + short_blocks) * slabs);
+  const int c = blockIdx.x % slabs * 32 * N + lane * W, block = blockIdx.x / slabs;
+  float acc[N];
   // Adds the shares of the chunks own + first, own + first + stride, ... (kUnroll of them at
   // most) of the run that begins in chunk `own`; whether the last of them belongs to it.
-  auto add = [&](float (&acc)[N], Item join, long long first, int stride) {
+  auto add = [&](Item join, long long first, int stride) {
     const long long own = join.place;
     Pack<float, N, W> v[kUnroll];
     bool on[kUnroll];
@@ -239,44 +273,36 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, 
       for (int e = 0; e < N; ++e) acc[e] += on[u] ? v[u].get(e) : 0.f;
     return on[kUnroll - 1];
   };
-  for (int first = blockIdx.x * kJoinWarps; first < most; first += gridDim.x * kJoinWarps) {
-    const int work = *join_count;
-    if (first >= work) return;
-    const Item join = joins[min(first + warp, most - 1)];  // read beside the count, not after it: there is room for `most`
-    bool longer = false;
-    float acc[N];
+  auto clear_sum = [&] {
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.f;
-    if (first + warp < work) {
-      static_assert(kUnroll == kShortRun);
-      const long long next = (long long)join.place + kShortRun;
-      longer = next * chunk < n && items[next * chunk].token == join.token;
-      if (!longer) {
-        add(acc, join, 0, 1);
-        if (c < width) write_sum<O, N, W>(out + (long long)join.token * out_stride, c, 32 * W, width, acc, scale, accumulate);
-      }
+  };
+  if (block >= long_blocks) {
+    for (int i = (block - long_blocks) * kJoinWarps + warp; i < chunks; i += short_blocks * kJoinWarps) {
+      const Item join = joins.shorter[i];  // read beside the count, not after it: there is room for all chunks
+      if (i >= joins.count[0]) return;
+      clear_sum();
+      add(join, 0, 1);
+      if (c < width) write_sum<O, N, W>(out + (long long)join.token * out_stride, c, 32 * W, width, acc, scale, accumulate);
     }
-    if (!__syncthreads_or(longer)) continue;
-    if (lane == 0) is_long[warp] = longer;
+    return;
+  }
+  for (int i = block; i < chunks; i += long_blocks) {
+    const Item join = joins.longer[i];
+    if (i >= joins.count[1]) return;
+    clear_sum();
+    for (long long j = warp; add(join, j, kJoinWarps); j += kJoinWarps * kUnroll) {
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) sums[warp][e * 32 + lane] = acc[e];
     __syncthreads();
-    for (int k = 0; k < kJoinWarps; ++k) {
-      if (!is_long[k]) continue;
-      const Item other = joins[first + k];
+    if (warp == 0 && c < width) {
+      for (int w = 1; w < kJoinWarps; ++w)
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] = 0.f;
-      for (long long j = warp; add(acc, other, j, kJoinWarps); j += kJoinWarps * kUnroll) {
-      }
-#pragma unroll
-      for (int e = 0; e < N; ++e) sums[warp][e * 32 + lane] = acc[e];
-      __syncthreads();
-      if (warp == 0 && c < width) {
-        for (int w = 1; w < kJoinWarps; ++w)
-#pragma unroll
-          for (int e = 0; e < N; ++e) acc[e] += sums[w][e * 32 + lane];
-        write_sum<O, N, W>(out + (long long)other.token * out_stride, c, 32 * W, width, acc, scale, accumulate);
-      }
-      __syncthreads();
+        for (int e = 0; e < N; ++e) acc[e] += sums[w][e * 32 + lane];
+      write_sum<O, N, W>(out + (long long)join.token * out_stride, c, 32 * W, width, acc, scale, accumulate);
     }
+    __syncthreads();
   }
 }
 
@@ -398,19 +424,24 @@ __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ gra
   }
 }
 
+// Bytes cleared beside the sort (about 15 us, at 6 TB/s) and beside the joins.
+constexpr long long kClearFirst = 96 << 20, kClearLast = 48 << 20;
+
 int chunk_of(long long n) { return n >= 16384 ? 32 : 16; }
 
 constexpr size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Workspace {
-  size_t a, b, join_count, joins, partial, bytes;
-  Workspace(long long n, int width) {
+  size_t a, b, join_count, shorter, longer, touched, partial, bytes;
+  Workspace(long long n, long long rows, int width) {
     const long long chunks = ceil_div_ll(n, chunk_of(n));
     a = 0;
     b = a + align_up(size_t(n) * sizeof(Item));
     join_count = b + align_up(size_t(n) * sizeof(Item));
-    joins = join_count + align_up(sizeof(int));
-    partial = joins + align_up(size_t(chunks) * sizeof(Item));
+    shorter = join_count + align_up(2 * sizeof(int));
+    longer = shorter + align_up(size_t(chunks) * sizeof(Item));
+    touched = longer + align_up(size_t(chunks) * sizeof(Item));
+    partial = touched + align_up(size_t(rows));
     bytes = partial + align_up(size_t(chunks) * 2 * size_t(width) * sizeof(float));
   }
 };
@@ -438,28 +469,38 @@ void embedding_launch(int dtype, RowsIn table, long long rows, int width, Indice
   PSB_LAUNCH_CHECK();
 }
 
-size_t embedding_grad_workspace(long long tokens, int width) { return tokens <= kFewTokens ? 0 : Workspace(tokens, width).bytes; }
+size_t embedding_grad_workspace(long long tokens, long long rows, int width) {
+  return tokens <= kFewTokens ? 0 : Workspace(tokens, rows, width).bytes;
+}
 
 void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float scale, long long padding, bool accumulate,
                            int out_dtype, RowsOut out, long long rows, int width, void* workspace, cudaStream_t stream) {
   const long long n = tokens.count;
   const int in_size = dtype_size(grad_dtype), out_size = dtype_size(out_dtype), chunk = chunk_of(n);
   if (n == 0 && accumulate) return;
-  const Workspace at(n, width);
+  const Workspace at(n, rows, width);
   char* ws = static_cast<char*>(workspace);
   auto* items = reinterpret_cast<Item*>(ws + at.a);
-  auto* joins = reinterpret_cast<Item*>(ws + at.joins);
-  auto* join_count = reinterpret_cast<int*>(ws + at.join_count);
+  const Joins joins{reinterpret_cast<Item*>(ws + at.shorter), reinterpret_cast<Item*>(ws + at.longer),
+                    reinterpret_cast<int*>(ws + at.join_count)};
   auto* partial = reinterpret_cast<float*>(ws + at.partial);
   const bool few = n <= kFewTokens;
   const long long row_bytes = (long long)width * out_size;
+  // A gradient of more than kClearFirst + kClearLast bytes is cleared in three parts, so
+  // that the sums and the joins, too, run beside a part of it.
+  const long long pitch = out.stride * out_size, first_rows = kClearFirst / row_bytes, last_rows = kClearLast / row_bytes;
+  const bool parts = !few && !accumulate && first_rows + last_rows < rows;
+  auto* touched = parts ? reinterpret_cast<unsigned char*>(ws + at.touched) : nullptr;
+  auto* bytes = static_cast<unsigned char*>(out.ptr);
+  const Rest middle{bytes, touched, first_rows, parts ? rows - last_rows : first_rows, row_bytes, pitch};
+  const Rest last{bytes, touched, middle.end, parts ? rows : middle.end, row_bytes, pitch};
   if (!few) {
-    const Clear zeros(out.ptr, rows, row_bytes, out.stride * out_size);
+    const Clear zeros(out.ptr, parts ? first_rows : rows, row_bytes, pitch);
     const int bits = bits_for((unsigned long long)rows), passes = ceil_div(bits, kMaxBits), pass_bits = ceil_div(bits, passes);
     const int blocks = sort_blocks(n);
     const long long clusters = 1 + (accumulate ? 0 : ceil_div_ll(zeros.blocks(), blocks));
     launch_clusters<embedding_order>(blocks, clusters, 1 << pass_bits, stream, tokens.ptr, tokens.wide, n, rows, padding, pass_bits,
-                                     passes, items, reinterpret_cast<Item*>(ws + at.b), chunk, joins, join_count, zeros);
+                                     passes, items, reinterpret_cast<Item*>(ws + at.b), chunk, joins, touched, zeros);
   }
   auto run = [&](auto t, auto o) {
     using T = decltype(t);
@@ -479,15 +520,20 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
         PSB_LAUNCH_CHECK();
         return;
       }
-      const unsigned chunks = grid_x(ceil_div_ll(n, chunk));
+      const int chunks = int(ceil_div_ll(n, chunk));
       // As few blocks a row as kSumThreads allows, and no more warps in them than the row fills.
       const int slabs = ceil_div(width, kSumThreads * N), threads = ceil_div(ceil_div(width, slabs * N), 32) * 32;
-      launch_after(sum_runs<T, O, N, W>, dim3(chunks, unsigned(slabs)), threads, stream, static_cast<const T*>(grad.ptr), grad.stride, items, n,
-                   uint32_t(rows), width, scale, accumulate, dst, out.stride, chunk, partial);
-      if (chunks == 1) return;
-      const dim3 joining(unsigned(std::min(ceil_div(int(chunks) - 1, kJoinWarps), 8 * device_sms())), unsigned(ceil_div(width, 32 * N)));
-      launch_after(join_runs<O, N, W>, joining, kJoinWarps * 32, stream, items, n, width, scale, accumulate, dst, out.stride, chunk,
-                   partial, joins, join_count, int(chunks) - 1);
+      const long long sum_blocks = (long long)chunks * slabs;
+      launch_after(sum_runs<T, O, N, W>, grid_x(sum_blocks + middle.blocks()), threads, stream, static_cast<const T*>(grad.ptr),
+                   grad.stride, items, n, uint32_t(rows), width, scale, accumulate, dst, out.stride, chunk, partial, int(sum_blocks),
+                   slabs, middle);
+      // At most one run in kShortRun chunks is long; few are.
+      const int join_slabs = ceil_div(width, 32 * N);
+      const int long_blocks = std::min(ceil_div(chunks, kShortRun), 32);
+      const int short_blocks = std::min(ceil_div(chunks, kJoinWarps), std::max(1, 8 * device_sms() / join_slabs));
+      launch_after(join_runs<O, N, W>, grid_x((long long)(long_blocks + short_blocks) * join_slabs + last.blocks()), kJoinWarps * 32,
+                   stream, items, n, width, scale, accumulate, dst, out.stride, chunk, partial, joins, chunks, long_blocks,
+                   short_blocks, join_slabs, last);
     });
   };
   with_type(grad_dtype, [&](auto t) {

@@ -33,7 +33,7 @@ constexpr int kMaxTopK = 32;       // a warp keeps one choice a lane
 void embedding_launch(int dtype, RowsIn table, long long rows, int width, Indices tokens, float scale, RowsOut out,
                       cudaStream_t stream);
 
-size_t embedding_grad_workspace(long long tokens, int width);
+size_t embedding_grad_workspace(long long tokens, long long rows, int width);
 void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float scale, long long padding, bool accumulate,
                            int out_dtype, RowsOut out, long long rows, int width, void* workspace, cudaStream_t stream);
 

@@ -153,7 +153,7 @@ def test_embedding_grad(dtype, out, width):
 
 
 @pytest.mark.parametrize("kind", ["any", "skewed", "one", "distinct", "sorted", "empty"])
-@pytest.mark.parametrize("n,rows", [(31, 9), (65, 5000), (2047, 300), (2048, 40000), (20000, 40000), (70001, 70001), (16384, 1025), (40000, 2_000_000), (9000, 512), (2049, 1023)])
+@pytest.mark.parametrize("n,rows", [(31, 9), (65, 5000), (2047, 300), (2048, 40000), (20000, 40000), (70001, 70001), (16384, 1025), (40000, 3_000_000), (9000, 512), (2049, 1023)])
 def test_embedding_grad_order_of_large_batches(kind, n, rows):
     g = gen(n + rows)
     if kind == "distinct" and n > rows:
@@ -163,6 +163,31 @@ def test_embedding_grad_order_of_large_batches(kind, n, rows):
     got = psb.embedding_grad(grad, tokens, rows, dtype=F32)
     check(got, want, slack)
     assert torch.equal(got, psb.embedding_grad(grad, tokens, rows, dtype=F32))  # the same bits again
+
+
+@pytest.mark.parametrize("n,chunk", [(2100, 16), (20000, 32)])
+@pytest.mark.parametrize("lengths", [(1, 15, 16, 17), (16, 32, 48), (31, 33, 1), (30, 2, 32, 1), (47, 17, 1), (64, 63, 65, 1), (200, 5), (33,)])
+def test_embedding_grad_of_runs_about_the_chunks_borders(n, chunk, lengths):
+    """Runs of every length about one, two and more chunks of the sorted batch, begun at every place in a chunk."""
+    g = gen(n)
+    runs = torch.tensor(lengths * (n // sum(lengths) + 1), device="cuda")
+    tokens = torch.repeat_interleave(torch.arange(len(runs), device="cuda"), runs)[:n]
+    tokens = tokens[torch.randperm(n, generator=g, device="cuda")]
+    tokens = torch.where(tokens % 5 == 4, tokens + len(runs), tokens)  # some outside
+    grad = randn(g, n, 40, dtype=BF16)
+    want, slack = grad64(grad, tokens, len(runs), 1.0)
+    check(psb.embedding_grad(grad, tokens, len(runs), dtype=F32), want, slack)
+
+
+def test_embedding_grad_of_a_large_table_with_rows_apart():
+    """The gradient that is cleared in parts (above 144 MiB), in a wider buffer whose other columns stay."""
+    g = gen(3)
+    tokens, grad = batch(g, "skewed", 5000, 300_000), randn(g, 5000, 130)
+    buf = torch.full((300_000, 133), 7.0, device="cuda")
+    psb.embedding_grad(grad, tokens, 300_000, out=buf[:, 1:131])
+    want, slack = grad64(grad, tokens, 300_000, 1.0)
+    check(buf[:, 1:131], want, slack)
+    assert (buf[:, 0] == 7).all() and (buf[:, 131:] == 7).all()
 
 
 def test_embedding_grad_of_a_million_tokens_and_many_passes():
