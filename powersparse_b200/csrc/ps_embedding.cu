@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kRowThreads) embedding_rows(const T* __restric
     for (int u = 0; u < kRowUnroll; ++u) {
 #pragma unroll
       for (int e = 0; e < N; ++e) v[u].set(e, v[u].get(e) * scale);
-      v[u].store(dst, c + u * lanes * N, step, width);
+      v[u].store_once(dst, c + u * lanes * N, step, width);
     }
   }
 }
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
     Item* out = to_a ? a : b;
     const Item* in = to_a ? b : a;
     const int shift = pass * pass_bits;
-    sort_pass<Item>(
+    sort_pass<Item, false>(
         sh, digits, pass & 1, strip,
         [&](long long i) -> Item {
           if (pass) return in[i];

@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kSortThreads) expert_order(const void* __restr
     return e >= 0 && e < experts ? int(e) : -1;
   };
   auto widen = [&](uint32_t count) { return (count + uint32_t(align) - 1) / uint32_t(align) * uint32_t(align); };
-  sort_pass<int>(
+  sort_pass<int, true>(
       SortShared(smem, experts), experts, 0, warp_strip(n, rank, blocks), expert, [](int e) { return e; }, widen,
       [&](int e, uint32_t begin, uint32_t count) {
         if (rank != 0) return;
@@ -318,7 +318,7 @@ __device__ __forceinline__ void copy_row(const unsigned char* x, const int* posi
       auto* dst = reinterpret_cast<Word<B>*>(out + p * out_bytes);
 #pragma unroll
       for (int u = 0; u < kRowUnroll; ++u)
-        if (c + u * lanes < words) dst[c + u * lanes] = v[u];
+        if (c + u * lanes < words) __stcs(dst + c + u * lanes, v[u]);
     }
   }
 }

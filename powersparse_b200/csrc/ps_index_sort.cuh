@@ -113,9 +113,10 @@ inline size_t sort_smem(int digits) { return sizeof(uint32_t) * ((kSortWarps + 3
 // stable order by digit.  load(i) gives the element i, digit_of(element) its digit (-1:
 // the element is not counted, and p means nothing).  widen(count) is the room that the
 // elements of a digit take (at least count); report(d, begin, count) is called by one
-// thread a digit in every block.  digits <= kMaxDigits.  Ends with the
-// cluster's barrier.
-template <typename Element, typename Load, typename DigitOf, typename Widen, typename Report, typename Place>
+// thread a digit in every block.  digits <= kMaxDigits.  kLast: nothing follows that
+// needs what the pass places; else it ends with the cluster's barrier, and `parity`
+// alternates from pass to pass.
+template <typename Element, bool kLast, typename Load, typename DigitOf, typename Widen, typename Report, typename Place>
 __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity, Strip strip, Load&& load, DigitOf&& digit_of,
                                           Widen&& widen, Report&& report, Place&& place) {
   namespace cg = cooperative_groups;
@@ -171,6 +172,9 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
       count += c;
     }
   }
+  // No block may end while another reads its totals: where no barrier follows at once,
+  // its two halves stand apart.
+  if (kLast && blocks > 1) cluster.barrier_arrive();
   const uint32_t begin = block_sum_before(d < digits ? widen(count) : 0u, sh.scratch);
   if (d < digits) {
     report(d, begin, count);
@@ -204,9 +208,8 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
       }
     }
   }
-  // The places are visible to the cluster, and no block ends (or counts again) while
-  // another may read its totals.
-  sort_barrier(blocks);
+  if (!kLast) sort_barrier(blocks);
+  else if (blocks > 1) cluster.barrier_wait();
 }
 
 // Blocks of the cluster for n indices: one while each warp's strip is short, more as

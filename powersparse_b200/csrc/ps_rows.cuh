@@ -75,6 +75,15 @@ struct Pack {
 #pragma unroll
         for (int k = 0; k < kParts; ++k) reinterpret_cast<Part*>(row + c + i * step)[k] = w[i][k];
   }
+  // For what this kernel does not read again: it makes room in the caches first (2% of
+  // the time of a large lookup or dispatch; the same for loads gained nothing).
+  __device__ __forceinline__ void store_once(T* row, int c, int step, int width) const {
+#pragma unroll
+    for (int i = 0; i < N / W; ++i)
+      if (c + i * step < width)
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) __stcs(reinterpret_cast<Part*>(row + c + i * step) + k, w[i][k]);
+  }
   // The same elements one at a time, for rows that do not allow the words.
   __device__ __forceinline__ void load_elements(const T* row, int c, int step, int width) {
 #pragma unroll
