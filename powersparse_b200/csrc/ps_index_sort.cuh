@@ -164,12 +164,13 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
 
   uint32_t count = 0, earlier = 0;
   if (d < digits) {
+    uint32_t c[kSortBlocks];  // all loads before their sum
+#pragma unroll
+    for (int b = 0; b < kSortBlocks; ++b) c[b] = b < blocks ? cluster.map_shared_rank(sh.total, b)[parity * digits + d] : 0u;
 #pragma unroll
     for (int b = 0; b < kSortBlocks; ++b) {
-      if (b >= blocks) break;
-      const uint32_t c = cluster.map_shared_rank(sh.total, b)[parity * digits + d];
-      if (b < rank) earlier += c;
-      count += c;
+      if (b < rank) earlier += c[b];
+      count += c[b];
     }
   }
   // No block may end while another reads its totals: where no barrier follows at once,

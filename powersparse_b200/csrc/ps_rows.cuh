@@ -28,6 +28,14 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
+// An element's bits as the word of its size.
+__device__ __forceinline__ float from_bits(uint32_t w, float) { return __uint_as_float(w); }
+__device__ __forceinline__ __nv_bfloat16 from_bits(uint16_t w, __nv_bfloat16) { return __ushort_as_bfloat16(w); }
+__device__ __forceinline__ __half from_bits(uint16_t w, __half) { return __ushort_as_half(w); }
+__device__ __forceinline__ uint32_t to_bits(float x) { return __float_as_uint(x); }
+__device__ __forceinline__ uint16_t to_bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+__device__ __forceinline__ uint16_t to_bits(__half x) { return __half_as_ushort(x); }
+
 // Words of B bytes: what one load or store moves.
 template <int B> struct WordOf;
 template <> struct WordOf<16> { using type = uint4; };
@@ -105,8 +113,15 @@ struct Pack {
 #pragma unroll
       for (int k = 0; k < kParts; ++k) w[i][k] = Part{};
   }
-  __device__ __forceinline__ float get(int e) const { return to_float(reinterpret_cast<const T*>(bytes)[e]); }
-  __device__ __forceinline__ void set(int e, float x) { reinterpret_cast<T*>(bytes)[e] = from_float<T>(x); }
+  // Single elements stay in registers of their own; in `bytes` two of 16 bits would share one.
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (W == 1) return to_float(from_bits(w[e][0], T()));
+    else return to_float(reinterpret_cast<const T*>(bytes)[e]);
+  }
+  __device__ __forceinline__ void set(int e, float x) {
+    if constexpr (W == 1) w[e][0] = to_bits(from_float<T>(x));
+    else reinterpret_cast<T*>(bytes)[e] = from_float<T>(x);
+  }
 };
 
 __device__ __forceinline__ long long index_at(const void* p, bool wide, long long i) {
