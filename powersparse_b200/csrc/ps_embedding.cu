@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
                                                                 long long rows, long long padding, int pass_bits, int passes,
                                                                 Item* a, Item* b, int chunk, Joins joins, unsigned char* touched,
                                                                 Clear zeros) {
-  extern __shared__ uint32_t smem[];
+  extern __shared__ __align__(16) unsigned char smem[];
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
     Item* out = to_a ? a : b;
     const Item* in = to_a ? b : a;
     const int shift = pass * pass_bits;
-    sort_pass<Item, false>(
+    sort_pass<Item, true, false>(
         sh, digits, pass & 1, strip,
         [&](long long i) -> Item {
           if (pass) return in[i];
@@ -499,7 +499,8 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
     const int bits = bits_for((unsigned long long)rows), passes = ceil_div(bits, kMaxBits), pass_bits = ceil_div(bits, passes);
     const int blocks = sort_blocks(n);
     const long long clusters = 1 + (accumulate ? 0 : ceil_div_ll(zeros.blocks(), blocks));
-    launch_clusters<embedding_order>(blocks, clusters, 1 << pass_bits, stream, tokens.ptr, tokens.wide, n, rows, padding, pass_bits,
+    const size_t smem = sort_smem(1 << pass_bits) + stage_smem(n, blocks, sizeof(Item));
+    launch_clusters<embedding_order>(blocks, clusters, smem, stream, tokens.ptr, tokens.wide, n, rows, padding, pass_bits,
                                      passes, items, reinterpret_cast<Item*>(ws + at.b), chunk, joins, touched, zeros);
   }
   auto run = [&](auto t, auto o) {

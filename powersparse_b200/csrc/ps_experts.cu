@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const floa
 __global__ void __launch_bounds__(kSortThreads) expert_order(const void* __restrict__ chosen, bool wide, long long n, int experts,
                                                              int align, int* __restrict__ position, int* __restrict__ offsets,
                                                              int* __restrict__ counts) {
-  extern __shared__ uint32_t smem[];
+  extern __shared__ __align__(16) unsigned char smem[];
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kSortThreads) expert_order(const void* __restr
     return e >= 0 && e < experts ? int(e) : -1;
   };
   auto widen = [&](uint32_t count) { return (count + uint32_t(align) - 1) / uint32_t(align) * uint32_t(align); };
-  sort_pass<int, true>(
+  sort_pass<int, false, true>(
       SortShared(smem, experts), experts, 0, warp_strip(n, rank, blocks), expert, [](int e) { return e; }, widen,
       [&](int e, uint32_t begin, uint32_t count) {
         if (rank != 0) return;
@@ -594,7 +594,7 @@ void dispatch_launch(int dtype, RowsIn x, Indices chosen, int tokens, int top_k,
   const long long row_bytes = (long long)width * size;
   const bool few = n <= kFewSlots;
   if (!few)
-    launch_clusters<expert_order>(sort_blocks(n), 1, experts, stream, chosen.ptr, chosen.wide, n, experts, align, position, offsets,
+    launch_clusters<expert_order>(sort_blocks(n), 1, sort_smem(experts), stream, chosen.ptr, chosen.wide, n, experts, align, position, offsets,
                                   counts);
   auto run = [&](auto bytes) {
     constexpr int B = decltype(bytes)::value;

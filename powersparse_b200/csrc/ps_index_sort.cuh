@@ -32,7 +32,8 @@ constexpr int kKeep = 8;
 constexpr int kSortBlocks = 16;    // the largest cluster there is (above 8 it needs an opt-in)
 
 struct Strip {
-  long long begin, end;
+  long long begin, end;  // of this warp
+  long long length, n;   // of every strip but the last ones, and of all
 };
 
 // The strip of this warp: 32-element chunks in order, the same number for every warp.
@@ -40,7 +41,7 @@ __device__ __forceinline__ Strip warp_strip(long long n, int rank, int blocks) {
   const long long warps = (long long)blocks * kSortWarps;
   const long long len = ((n + warps - 1) / warps + 31) / 32 * 32;
   const long long b = (rank * (long long)kSortWarps + (threadIdx.x >> 5)) * len;
-  return {b < n ? b : n, b + len < n ? b + len : n};
+  return {b < n ? b : n, b + len < n ? b + len : n, len, n};
 }
 
 // row[d] of the lanes' digits d (-1: none) before this chunk of 32, plus the number of
@@ -65,29 +66,31 @@ __device__ __forceinline__ uint32_t rank_chunk(uint32_t* row, int d, int bits) {
   return first + __popc(same & ((1u << lane) - 1u));
 }
 
-// Exclusive sum over the block's threads; `scratch` holds kSortWarps words.
-__device__ __forceinline__ uint32_t block_sum_before(uint32_t v, uint32_t* scratch) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t inc = v;
+// Exclusive sums of two numbers over the block's threads; `scratch` holds kSortWarps pairs.
+__device__ __forceinline__ uint2 warp_sums(uint2 v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const uint32_t o = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += o;
+    const uint32_t x = __shfl_up_sync(0xffffffffu, v.x, d), y = __shfl_up_sync(0xffffffffu, v.y, d);
+    if (lane >= d) {
+      v.x += x;
+      v.y += y;
+    }
   }
+  return v;
+}
+__device__ __forceinline__ uint2 block_sums_before(uint2 v, uint2* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint2 inc = warp_sums(v);
   if (lane == 31) scratch[warp] = inc;
   __syncthreads();
+  static_assert(kSortWarps == 32);
   if (warp == 0) {
-    const uint32_t w = lane < kSortWarps ? scratch[lane] : 0u;
-    uint32_t winc = w;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t o = __shfl_up_sync(0xffffffffu, winc, d);
-      if (lane >= d) winc += o;
-    }
-    if (lane < kSortWarps) scratch[lane] = winc - w;
+    const uint2 w = scratch[lane], all = warp_sums(w);
+    scratch[lane] = make_uint2(all.x - w.x, all.y - w.y);
   }
   __syncthreads();
-  return scratch[warp] + inc - v;
+  return make_uint2(scratch[warp].x + inc.x - v.x, scratch[warp].y + inc.y - v.y);
 }
 
 // The cluster's barrier; a cluster of one block needs only the block's.
@@ -97,26 +100,41 @@ __device__ __forceinline__ void sort_barrier(int blocks) {
 }
 
 // Shared memory of a sort: kSortWarps rows of counters, two sets of block totals (one
-// pass writes one while a slower block may still read the other), the digits' bases
-// and scratch.
+// pass writes one while a slower block may still read the other), the digits' bases,
+// the digits' first places among the block's staged elements, and scratch; then the
+// staged elements.
 struct SortShared {
-  uint32_t* rows;
-  uint32_t* total;
-  uint32_t* base;
-  uint32_t* scratch;
-  __device__ SortShared(uint32_t* smem, int digits)
-      : rows(smem), total(smem + kSortWarps * digits), base(total + 2 * digits), scratch(base + digits) {}
+  uint2* scratch;
+  uint32_t *rows, *total, *base, *local;
+  void* stage;
+  __device__ SortShared(void* smem, int digits)
+      : scratch(static_cast<uint2*>(smem)),
+        rows(reinterpret_cast<uint32_t*>(scratch + kSortWarps)),
+        total(rows + kSortWarps * digits),
+        base(total + 2 * digits),
+        local(base + digits),
+        stage(local + digits) {}
 };
-inline size_t sort_smem(int digits) { return sizeof(uint32_t) * ((kSortWarps + 3) * size_t(digits) + kSortWarps); }
+inline size_t sort_smem(int digits) {
+  return kSortWarps * sizeof(uint2) + sizeof(uint32_t) * ((kSortWarps + 4) * (size_t(digits) + (digits & 1)));
+}
+// Bytes of the staged elements of n indices in `blocks` blocks (none where the strips are walked twice).
+inline size_t stage_smem(long long n, int blocks, size_t element) {
+  const long long strip = ceil_div_ll(ceil_div_ll(n, (long long)blocks * kSortWarps), 32) * 32;
+  return strip <= kKeep * 32 ? size_t(strip) * kSortWarps * element : 0;
+}
 
 // One pass: place(i, element, p) for every element of the strip, p its position in the
 // stable order by digit.  load(i) gives the element i, digit_of(element) its digit (-1:
 // the element is not counted, and p means nothing).  widen(count) is the room that the
 // elements of a digit take (at least count); report(d, begin, count) is called by one
-// thread a digit in every block.  digits <= kMaxDigits.  kLast: nothing follows that
+// thread a digit in every block.  digits <= kMaxDigits.  kStage: elements that are kept
+// are put in order in shared memory first and placed from there, so that a warp's
+// places lie side by side: for elements that place() moves (8 bytes to scattered places
+// leave an SM at one in 2.5 cycles: 50003 of them took 4 us a pass).  kLast: nothing follows that
 // needs what the pass places; else it ends with the cluster's barrier, and `parity`
 // alternates from pass to pass.
-template <typename Element, bool kLast, typename Load, typename DigitOf, typename Widen, typename Report, typename Place>
+template <typename Element, bool kStage, bool kLast, typename Load, typename DigitOf, typename Widen, typename Report, typename Place>
 __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity, Strip strip, Load&& load, DigitOf&& digit_of,
                                           Widen&& widen, Report&& report, Place&& place) {
   namespace cg = cooperative_groups;
@@ -128,7 +146,10 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
   for (int d = lane; d < digits; d += 32) row[d] = 0;
   __syncwarp();
 
-  const bool kept = strip.end - strip.begin <= kKeep * 32;
+  // Every warp's strip is as long, but for the last ones.
+  const bool kept = strip.length <= kKeep * 32;
+  const long long block_begin = min(strip.n, strip.length * kSortWarps * rank);
+  const long long block_end = min(strip.n, block_begin + strip.length * kSortWarps);
   Element e[kKeep];
   uint32_t r[kKeep];
   for (long long base = strip.begin; base < strip.end; base += kKeep * 32) {
@@ -162,8 +183,9 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
   }
   sort_barrier(blocks);
 
-  uint32_t count = 0, earlier = 0;
+  uint32_t count = 0, earlier = 0, own = 0;
   if (d < digits) {
+    own = sh.total[parity * digits + d];
     uint32_t c[kSortBlocks];  // all loads before their sum
 #pragma unroll
     for (int b = 0; b < kSortBlocks; ++b) c[b] = b < blocks ? cluster.map_shared_rank(sh.total, b)[parity * digits + d] : 0u;
@@ -176,14 +198,30 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
   // No block may end while another reads its totals: where no barrier follows at once,
   // its two halves stand apart.
   if (kLast && blocks > 1) cluster.barrier_arrive();
-  const uint32_t begin = block_sum_before(d < digits ? widen(count) : 0u, sh.scratch);
+  const uint2 begin = block_sums_before(make_uint2(d < digits ? widen(count) : 0u, own), sh.scratch);
+  const bool staged = kStage && kept;
   if (d < digits) {
-    report(d, begin, count);
-    sh.base[d] = begin + earlier;
+    report(d, begin.x, count);
+    sh.base[d] = begin.x + earlier - (staged ? begin.y : 0u);
+    if (staged) sh.local[d] = begin.y;
   }
   __syncthreads();
 
-  if (kept) {
+  if (staged) {
+    auto* stage = static_cast<Element*>(sh.stage);
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u)
+      if (strip.begin + u * 32 + lane < strip.end) {
+        const int digit = digit_of(e[u]);
+        stage[sh.local[digit] + row[digit] + r[u]] = e[u];
+      }
+    __syncthreads();
+    const int mine = int(block_end - block_begin);
+    for (int i = threadIdx.x; i < mine; i += kSortThreads) {
+      const Element element = stage[i];
+      place(i, element, sh.base[digit_of(element)] + i);
+    }
+  } else if (kept) {
 #pragma unroll
     for (int u = 0; u < kKeep; ++u) {
       const long long i = strip.begin + u * 32 + lane;
@@ -240,14 +278,15 @@ void launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_
 }
 
 // Launches `kernel` with `clusters` clusters of `blocks` blocks of kSortThreads.
+constexpr int kSortSmem = 220 << 10;  // what the most digits and the longest kept strips of 8-byte elements take, and some
 template <auto kernel, typename... Args>
-void launch_clusters(int blocks, long long clusters, int digits, cudaStream_t stream, Args... args) {
+void launch_clusters(int blocks, long long clusters, size_t smem, cudaStream_t stream, Args... args) {
   static std::atomic<unsigned long long> prepared{0};  // devices on which the kernel may take its largest shared memory
   int device = 0;
   PSB_CUDA(cudaGetDevice(&device));
   const unsigned long long bit = device < 64 ? 1ULL << device : 0;
   if (!(prepared.load(std::memory_order_relaxed) & bit)) {
-    PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sort_smem(kMaxDigits))));
+    PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem));
     PSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     prepared.fetch_or(bit, std::memory_order_relaxed);
   }
@@ -255,7 +294,7 @@ void launch_clusters(int blocks, long long clusters, int digits, cudaStream_t st
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(clusters * blocks));
   config.blockDim = dim3(kSortThreads);
-  config.dynamicSmemBytes = sort_smem(digits);
+  config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attr[1] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
