@@ -90,12 +90,14 @@ struct Clear {
 struct Rest {
   unsigned char* ptr;
   const unsigned char* touched;
-  long long begin, end, bytes, pitch;
-  static constexpr int kBytes = 1 << 16;  // of a block
-  __host__ __device__ long long block_rows() const { return bytes >= kBytes ? 1 : kBytes / bytes; }
-  __host__ long long blocks() const { return ceil_div_ll(end - begin, block_rows()); }
+  long long begin, end, bytes, pitch, block_rows;
+  // By blocks of `warps` warps, each of one row at least and about 64 KiB.
+  Rest(unsigned char* p, const unsigned char* t, long long b, long long e, long long row_bytes, long long row_pitch, int warps)
+      : ptr(p), touched(t), begin(b), end(e), bytes(row_bytes), pitch(row_pitch),
+        block_rows(std::max<long long>(warps, (1 << 16) / row_bytes)) {}
+  __host__ long long blocks() const { return ceil_div_ll(end - begin, block_rows); }
   __device__ void run(long long block) const {
-    const long long first = begin + block * block_rows(), last = min(end, first + block_rows());
+    const long long first = begin + block * block_rows, last = min(end, first + block_rows);
     for (long long r = first + (threadIdx.x >> 5); r < last; r += blockDim.x >> 5)
       if (!touched[r]) clear(ptr + r * pitch, bytes, threadIdx.x & 31, 32);
   }
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
 // partial rows: [0] for the run that began before the chunk, [1] for one that goes on
 // after it.  join_runs adds those up.
 constexpr int kSumThreads = 128;
-constexpr int kMaxChunk = 32;
+constexpr int kMaxChunk = 64;
 
 template <typename O, int N, int W>
 __device__ __forceinline__ void write_sum(O* row, int c, int step, int width, const float (&acc)[N], float scale, bool accumulate) {
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
 // The runs that cross a border, 32 * N columns at a time.  Blocks first take the longer
 // ones, all their warps one run (every kJoinWarps-th chunk each, then over the warps);
 // the `short_blocks` behind them take a short one a warp.
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 16;
 
 template <typename O, int N, int W>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, long long n, int width, float scale,
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ gra
 // Bytes cleared beside the sort (about 15 us, at 6 TB/s) and beside the joins.
 constexpr long long kClearFirst = 96 << 20, kClearLast = 48 << 20;
 
-int chunk_of(long long n) { return n >= 16384 ? 32 : 16; }
+int chunk_of(long long n) { return n >= 32768 ? 64 : n >= 16384 ? 32 : 16; }
 
 constexpr size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 
@@ -492,8 +494,8 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
   const bool parts = !few && !accumulate && first_rows + last_rows < rows;
   auto* touched = parts ? reinterpret_cast<unsigned char*>(ws + at.touched) : nullptr;
   auto* bytes = static_cast<unsigned char*>(out.ptr);
-  const Rest middle{bytes, touched, first_rows, parts ? rows - last_rows : first_rows, row_bytes, pitch};
-  const Rest last{bytes, touched, middle.end, parts ? rows : middle.end, row_bytes, pitch};
+  const Rest middle{bytes, touched, first_rows, parts ? rows - last_rows : first_rows, row_bytes, pitch, kSumThreads / 32};
+  const Rest last{bytes, touched, middle.end, parts ? rows : middle.end, row_bytes, pitch, kJoinWarps};
   if (!few) {
     const Clear zeros(out.ptr, parts ? first_rows : rows, row_bytes, pitch);
     const int bits = bits_for((unsigned long long)rows), passes = ceil_div(bits, kMaxBits), pass_bits = ceil_div(bits, passes);
