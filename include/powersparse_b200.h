@@ -223,9 +223,10 @@ int ps_partition_rows(int row_num, const int* row_ptr, int parts, int* cuts);
  * run on the current device, asynchronously on `stream`.  A matrix argument is rows
  * of `width` elements of type `dtype`, `stride` elements apart (stride >= width,
  * width <= 2^24); byte offsets are 64-bit.  Sums, products and softmax statistics
- * are FP32, rounded once, to nearest even, where they are stored.  No call allocates
- * device memory, waits for the device or uses atomics whose order matters: equal
- * inputs give equal bits, and every call can be captured into a graph.  Rows that
+ * are FP32, rounded once, to nearest even, where they are stored.  An output must not
+ * overlap an input but where it is said.  No call allocates device memory, waits for
+ * the device or uses atomics whose order matters: equal inputs at equal alignment give
+ * equal bits, and every call can be captured into a graph.  Rows that
  * begin at multiples of 16 bytes, with a width that is a multiple of 16 bytes, are
  * moved 16 bytes a thread; others by smaller words. */
 enum { PS_F32 = 0, PS_BF16 = 1, PS_F16 = 2 }; /* element types */
@@ -245,8 +246,8 @@ int ps_embedding(const void* table, int dtype, long long rows, int width, long l
  * grad_table's type is grad's or PS_F32.  rows <= 2^31 - 2.  workspace: at least
  * ps_embedding_grad_workspace(n, rows, width) bytes of device memory at a multiple
  * of 256 (-1 for arguments out of range; 0 for small batches, where it may be NULL),
- * in use until the call has run; it needs no initialisation and nothing in it
- * outlives the call. */
+ * in use until the call has run (by a graph that captured the call, while the graph
+ * may run); it needs no initialisation and nothing in it outlives the call. */
 long long ps_embedding_grad_workspace(long long n, long long rows, int width);
 int ps_embedding_grad(const void* grad, int grad_dtype, long long grad_stride, const void* tokens, int index_type, long long n,
                       float scale, long long padding, int accumulate, void* grad_table, int table_dtype, long long table_stride,
@@ -296,7 +297,7 @@ int ps_combine(const void* y, int dtype, long long y_stride, long long row_count
 
 /* Gradient of ps_combine for y and the weights: grad_y[position[t, j], :] = weights[t, j]
  * * grad[t, :], grad_weights[t, j] = <grad[t, :], y[position[t, j], :]> (0 for a skipped
- * position).  position, offsets and counts are ps_dispatch's: the rows between an
+ * position).  grad_y may be y itself.  position, offsets and counts are ps_dispatch's: the rows between an
  * expert's tokens and the next expert are set to zeros, and zero_tail says the same
  * of the rows from offsets[experts] on as there.  (The gradient for add is grad itself.) */
 int ps_combine_grad(const void* grad, int dtype, long long grad_stride, const void* y, long long y_stride, long long row_count,

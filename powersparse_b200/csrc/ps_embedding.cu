@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(kRowThreads) embedding_rows(const T* __restric
   const long long token = index_at(tokens, wide, i);
   const bool inside = token >= 0 && token < rows;
   const T* src = table + (inside ? token : 0) * table_stride;
+  if (!inside) scale = 0.f;  // +0, whatever the scale
   T* dst = out + i * out_stride;
   for (int c = first_column<N, W, S>(threadIdx.x & (lanes - 1)); c < width; c += lanes * N * kRowUnroll) {
     Pack<T, N, W> v[kRowUnroll];
@@ -312,7 +313,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, 
 // A block for every token of the batch: the first of its kind adds up all of them (the
 // others end), in the order of the batch.  Up to kFewTokens / kFewThreads tokens a
 // thread are compared, so no sort is needed, and neither are partial rows.  Behind them
-// the blocks that clear the rows which no token names.
+// the blocks that clear the rows which no token names.  Against the sort and its
+// launches: 1024 tokens, rows of 256, 10.3 us against 18.5; 2048 tokens 14.1 against
+// 20.9 (rows of 2048: 24.5 against 22.7); 4096 tokens 34 against 21, as every block
+// reads every token.
 constexpr int kFewTokens = 2048;
 constexpr int kFewThreads = 256;
 constexpr int kFewEach = kFewTokens / kFewThreads;
@@ -429,6 +433,9 @@ __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ gra
 // Bytes cleared beside the sort (about 15 us, at 6 TB/s) and beside the joins.
 constexpr long long kClearFirst = 96 << 20, kClearLast = 48 << 20;
 
+// Sorted positions a block adds up: more of them make fewer partial rows and joins, but
+// fewer blocks.  64 against 32: 65536 tokens in rows of 1024 64 against 71 us; 16384
+// tokens in rows of 2048 188 against 180.
 int chunk_of(long long n) { return n >= 32768 ? 64 : n >= 16384 ? 32 : 16; }
 
 constexpr size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
@@ -509,7 +516,9 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
     using T = decltype(t);
     using O = decltype(o);
     auto fits = [&](int bytes) {
-      return rows_aligned(grad.ptr, grad.stride, in_size, bytes) && rows_aligned(out.ptr, out.stride, out_size, bytes);
+      // A word of the gradient of the table has as many elements, not as many bytes.
+      return rows_aligned(grad.ptr, grad.stride, in_size, bytes) &&
+             rows_aligned(out.ptr, out.stride, out_size, std::min(16, bytes / in_size * out_size));
     };
     with_shape<T>(width, fits, [&](auto shape) {
       constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;

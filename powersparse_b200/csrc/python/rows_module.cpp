@@ -194,8 +194,13 @@ class Place {
     if (stream == Py_None) {
       handle_ = c10::cuda::getCurrentCUDAStream(device.index()).stream();
     } else {
-      handle_ = reinterpret_cast<cudaStream_t>(integer(stream, "stream"));
-      stream_.emplace(c10::cuda::getStreamFromExternal(handle_, device.index()));
+      const int64_t value = integer(stream, "stream");
+      // 0 and cudaStreamLegacy are the default stream; torch takes other odd values for streams of its own.
+      if (value != 0 && value != 1 && value % 2) refuse("stream is not a stream's handle");
+      const auto s = value == 0 || value == 1 ? c10::cuda::getDefaultCUDAStream(device.index())
+                                              : c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(value), device.index());
+      handle_ = s.stream();
+      stream_.emplace(s);
     }
   }
   void* handle() const { return handle_; }

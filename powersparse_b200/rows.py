@@ -14,8 +14,10 @@ stride of at least the width); indices are int32 or int64.  ``stream`` is a torc
 stream or a raw handle; without it a call runs on PyTorch's current stream of the
 tensors' device, which need not be the current device.  With it, outputs and scratch
 that the call allocates belong to that stream, and ordering the inputs before it and
-other uses of the outputs after it is the caller's part, as with SpMM.  Nothing here
-waits for the device, and every call can be captured into a CUDA graph.
+other uses of the outputs after it is the caller's part, as with SpMM.  An ``out`` must
+not overlap the inputs but where its function says so.  Nothing here waits for the
+device, and every call can be captured into a CUDA graph.  These functions take no part
+in autograd.
 
 The C entry points and their exact contracts are in ``include/powersparse_b200.h``.
 ``powersparse_b200.torch_ops`` registers the same operators, with autograd, as
@@ -150,6 +152,6 @@ def combine_grad(grad, y, plan, weights, out=None, stream=None):
     """``(grad_y, grad_weights)`` of ``combine`` (ps_combine_grad).
 
     Rows of ``grad_y`` that no token has are zeros.  ``out``: the tensor for ``grad_y``, [len(y), width], of which
-    the rows from ``plan.offsets[-1]`` on stay as they were.
+    the rows from ``plan.offsets[-1]`` on stay as they were; it may be ``y`` itself.
     """
     return _native.combine_grad(grad, y, *plan, weights, out, _handle(stream, y))

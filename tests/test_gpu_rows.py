@@ -7,6 +7,10 @@ m * u * sum |terms| to first order (products included); the factor 1.01 covers t
 higher orders (m * u < 1e-2 in every test).
 """
 import math
+import os
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -177,6 +181,27 @@ def test_embedding_grad_of_runs_about_the_chunks_borders(n, chunk, lengths):
     grad = randn(g, n, 40, dtype=BF16)
     want, slack = grad64(grad, tokens, len(runs), 1.0)
     check(psb.embedding_grad(grad, tokens, len(runs), dtype=F32), want, slack)
+
+
+@pytest.mark.parametrize("n", [100, 3000])
+@pytest.mark.parametrize("offset,extra", [(0, 0), (0, 1), (1, 0), (1, 1), (2, 2), (1, 3), (2, 6), (4, 4)])
+def test_embedding_grad_in_32_bits_at_every_alignment(n, offset, extra):
+    """16-bit rows that allow words while the 32-bit rows of the result begin elsewhere, and the other way round."""
+    g = gen(offset)
+    for width in (2, 6, 8, 64, 132):
+        tokens, grad = batch(g, "skewed", n, 70), randn(g, n, width, dtype=F16)
+        want, slack = grad64(grad, tokens, 70, 1.0)
+        for a, b in (((0, 0), (extra, offset)), ((extra, offset), (0, 0)), ((2, 2), (extra, offset))):
+            dst = strided(torch.full((70, width), 7.0, device="cuda"), *b)
+            psb.embedding_grad(strided(grad, *a), tokens, 70, out=dst)
+            check(dst, want, slack, (width, a, b))
+
+
+def test_empty_places_are_plus_zero_whatever_the_scale():
+    tokens = torch.tensor([-1, 3, 9], device="cuda")
+    for scale in (-1.5, math.inf, math.nan):
+        out = psb.embedding(torch.ones(9, 16, device="cuda"), tokens, scale)
+        assert (out[[0, 2]].view(torch.int32) == 0).all()
 
 
 def test_embedding_grad_of_a_large_table_with_rows_apart():
@@ -627,6 +652,95 @@ def test_replayed_graphs_streams_and_two_at_once():
         torch.cuda.synchronize()
         for out, i in zip(outs, rounds):
             assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+def test_capture_before_any_eager_call():
+    """In a process of its own, each operator's first call is a captured one."""
+    code = """
+import torch, sys
+sys.path.insert(0, %r)
+import test_gpu_rows as t
+s = t.inputs(1)
+many = t.inputs(2, 3000)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = t.run_all(s) + t.run_all(many)
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, t.run_all(s) + t.run_all(many)))
+print("captured first")
+""" % os.path.dirname(os.path.abspath(__file__))
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                         cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert "captured first" in run.stdout, run.stderr[-2000:]
+
+
+def test_training_step_captured_and_replayed():
+    """Forward and backward of the registered ops in a graph: gradients of each replay's inputs."""
+    g = gen(21)
+    vocab, width, experts, k, n = 40, 16, 4, 2, 24
+    table, gate = randn(g, vocab, width).requires_grad_(), (randn(g, width, experts) * 0.3).requires_grad_()
+    tokens = torch.randint(-1, vocab, (n,), generator=g, device="cuda")
+    ops = torch.ops.powersparse
+
+    def step():
+        h = ops.embedding(table, tokens, 1.5)
+        weights, chosen = ops.route(h @ gate, k, False)
+        rows, position, offsets, counts = ops.dispatch(h, chosen, experts, 8)
+        out = ops.combine(torch.tanh(rows), position, offsets, counts, weights, h)
+        return torch.autograd.grad((out * out).sum(), (table, gate))
+    want = []
+    batches = [torch.randint(-1, vocab, (n,), generator=g, device="cuda") for _ in range(3)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for b in batches:
+            tokens.copy_(b)
+            want.append([t.clone() for t in step()])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for b, w in zip(batches, want):
+        tokens.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        # The same kernels on the same numbers, but torch's products (16 and 24 terms of order one: off by 24 * u, under
+        # 2e-6, each; three lie on a path) may be made by another kernel.
+        assert all(torch.allclose(a, c, rtol=1e-5, atol=1e-5) for a, c in zip(got, w))
+
+
+def test_calls_from_two_threads():
+    sets = [inputs(s, 2500) for s in (1, 2)]
+    want = [run_all(s) for s in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = run_all(sets[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_default_stream_by_its_handles():
+    s = inputs(3)
+    torch.cuda.synchronize()
+    for handle in (0, 1):
+        out = psb.embedding(s["table"], s["tokens"], 2.0, stream=handle)
+        torch.cuda.synchronize()
+        assert torch.equal(out, psb.embedding(s["table"], s["tokens"], 2.0))
+    with pytest.raises(ValueError, match="handle"):
+        psb.embedding(s["table"], s["tokens"], stream=7)
 
 
 def test_explicit_stream_owns_what_the_call_allocates():
