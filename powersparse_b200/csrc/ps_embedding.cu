@@ -105,24 +105,14 @@ struct Rest {
 };
 
 // The first cluster sorts the tokens; tokens outside [0, rows) and the padding token
-// get the key `rows` and come last.  The sorted items are in `a`.  Then it lists the
-// chunks of sorted items in which a run of one token begins that goes on in the next
-// chunk, those of at most kShortRun chunks (at least two) and the longer ones apart, in any order.  The
-// other clusters clear the gradient meanwhile, or the first rows of a large one: rows
-// that no token names need it, and what the others cost is hidden, since the sort
-// leaves most of the GPU idle.  touched (null unless rows are left to the later
-// kernels): 1 for every token that occurs.
-constexpr int kShortRun = 4;
-
-struct Joins {
-  Item* shorter;  // token and chunk
-  Item* longer;
-  int* count;  // of the two
-};
-
+// get the key `rows` and come last.  The sorted items are in `a`.  The other clusters
+// clear the gradient meanwhile, or the first rows of a large one: rows that no token
+// names need it, and what the others cost is hidden, since the sort leaves most of the
+// GPU idle.  touched (null unless rows are left to the later kernels): 1 for every token
+// that occurs.  counts: two numbers to be set to zero.
 __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __restrict__ tokens, bool wide, long long n,
                                                                 long long rows, long long padding, int pass_bits, int passes,
-                                                                Item* a, Item* b, int chunk, Joins joins, unsigned char* touched,
+                                                                Item* a, Item* b, int* counts, unsigned char* touched,
                                                                 Clear zeros) {
   extern __shared__ __align__(16) unsigned char smem[];
   namespace cg = cooperative_groups;
@@ -133,7 +123,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
   const int digits = 1 << pass_bits;
   const SortShared sh(smem, digits);
   const Strip strip = warp_strip(n, rank, blocks);
-  if (rank == 0 && threadIdx.x < 2) joins.count[threadIdx.x] = 0;
+  if (rank == 0 && threadIdx.x < 2) counts[threadIdx.x] = 0;
   if (touched)
     for (long long v = rank * kSortThreads + threadIdx.x; v < rows; v += blocks * kSortThreads) touched[v] = 0;
   for (int pass = 0; pass < passes; ++pass) {
@@ -155,13 +145,6 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
           if (touched && pass == 0 && e.token < rows) touched[e.token] = 1;  // cleared before the barrier of the pass
         });
   }
-  for (long long c = rank * kSortThreads + threadIdx.x; (c + 1) * chunk < n; c += blocks * kSortThreads) {
-    const uint32_t token = a[(c + 1) * chunk - 1].token;
-    if (token < rows && a[(c + 1) * chunk].token == token && (c == 0 || a[c * chunk - 1].token != token)) {
-      const bool longer = (c + kShortRun) * chunk < n && a[(c + kShortRun) * chunk].token == token;
-      (longer ? joins.longer : joins.shorter)[atomicAdd(joins.count + longer, 1)] = {token, uint32_t(c)};
-    }
-  }
 }
 
 // ---- gradient: sums of the sorted rows ----------------------------------------------
@@ -169,7 +152,16 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
 // adds the gradient rows run by run in 32-bit registers.  A run inside the chunk goes
 // to its row; what belongs to a run that crosses a border goes to the chunk's two
 // partial rows: [0] for the run that began before the chunk, [1] for one that goes on
-// after it.  join_runs adds those up.
+// after it.  join_runs adds those up, by a list of the chunks in which such runs begin:
+// those of at most kShortRun chunks (at least two) and the longer ones apart, in any order.
+constexpr int kShortRun = 4;
+
+struct Joins {
+  Item* shorter;  // token and chunk
+  Item* longer;
+  int* count;  // of the two
+};
+
 constexpr int kSumThreads = 128;
 constexpr int kMaxChunk = 64;
 
@@ -187,7 +179,7 @@ template <typename T, typename O, int N, int W>
 __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ grad, long long grad_stride,
                                                         const Item* items, long long n, uint32_t rows, int width, float scale, bool accumulate,
                                                         O* __restrict__ out, long long out_stride, int chunk,
-                                                        float* __restrict__ partial, int sum_blocks, int slabs, Rest rest) {
+                                                        float* __restrict__ partial, Joins joins, int sum_blocks, int slabs, Rest rest) {
   constexpr int kUnroll = 8;
   constexpr uint32_t kNone = 0xffffffffu;
   __shared__ uint32_t key[kMaxChunk + 2], at[kMaxChunk];
@@ -203,6 +195,14 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
     if (i >= 1 && i <= count) at[i - 1] = item.place;
   }
   __syncthreads();
+  if (blockIdx.x % slabs == 0 && threadIdx.x == 0) {
+    const uint32_t token = key[count];
+    if (token < rows && key[count + 1] == token && !(key[0] == token && key[1] == token)) {  // begins here and goes on
+      const long long far = (block + kShortRun) * chunk;
+      const bool longer = far < n && items[far].token == token;
+      (longer ? joins.longer : joins.shorter)[atomicAdd(joins.count + longer, 1)] = {token, uint32_t(block)};
+    }
+  }
   constexpr int step = 32 * W;
   const int c = first_column<N, W, 32>(blockIdx.x % slabs * blockDim.x + threadIdx.x);
   if (c >= width) return;
@@ -510,7 +510,7 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
     const long long clusters = 1 + (accumulate ? 0 : ceil_div_ll(zeros.blocks(), blocks));
     const size_t smem = sort_smem(1 << pass_bits) + stage_smem(n, blocks, sizeof(Item));
     launch_clusters<embedding_order>(blocks, clusters, smem, stream, tokens.ptr, tokens.wide, n, rows, padding, pass_bits,
-                                     passes, items, reinterpret_cast<Item*>(ws + at.b), chunk, joins, touched, zeros);
+                                     passes, items, reinterpret_cast<Item*>(ws + at.b), joins.count, touched, zeros);
   }
   auto run = [&](auto t, auto o) {
     using T = decltype(t);
@@ -537,8 +537,8 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
       const int slabs = ceil_div(width, kSumThreads * N), threads = ceil_div(ceil_div(width, slabs * N), 32) * 32;
       const long long sum_blocks = (long long)chunks * slabs;
       launch_after(sum_runs<T, O, N, W>, grid_x(sum_blocks + middle.blocks()), threads, stream, static_cast<const T*>(grad.ptr),
-                   grad.stride, items, n, uint32_t(rows), width, scale, accumulate, dst, out.stride, chunk, partial, int(sum_blocks),
-                   slabs, middle);
+                   grad.stride, items, n, uint32_t(rows), width, scale, accumulate, dst, out.stride, chunk, partial, joins,
+                   int(sum_blocks), slabs, middle);
       // At most one run in kShortRun chunks is long; few are.
       const int join_slabs = ceil_div(width, 32 * N);
       const int long_blocks = std::min(ceil_div(chunks, kShortRun), 32);
