@@ -15,7 +15,9 @@ namespace psb {
 namespace {
 
 // ---- lookup ---------------------------------------------------------------------
-// 2^lanes_log2 threads a row, kRowUnroll words of it in flight each.
+// 2^lanes_log2 threads a row, kRowUnroll words of it in flight each.  Bound by memory:
+// 16384 tokens of 4096 in 16 bits take 31 us, 6.1 TB/s of the 189 MB that have to move;
+// 16 tokens 2.1 us, a launch.
 constexpr int kRowThreads = 256;
 constexpr int kRowUnroll = 4;
 
@@ -162,6 +164,11 @@ struct Joins {
   int* count;  // of the two
 };
 
+// Bound by memory where the rows are wide and the table large (16384 tokens of 2048 in
+// 16 bits into 131072 rows in 32: 176 us for sort, sums, joins and clearing together, 98%
+// of the copy rate).  Ragged rows (50003 of 515 in 16 bits, 43 us in all) are bound by
+// latency and instructions: 21 us for the sort's two passes, about 14 for the sums, 8
+// for the joins.
 constexpr int kSumThreads = 128;
 constexpr int kMaxChunk = 64;
 
