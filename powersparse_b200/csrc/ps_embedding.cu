@@ -67,23 +67,66 @@ __device__ __forceinline__ void clear(unsigned char* p, long long bytes, int thr
   for (long long i = thread; i < (bytes - head - words * 16) / 2; i += threads) tail[i] = 0;
 }
 
+// The same word by word for `rows` rows of `words` words, `pitch` bytes apart, but for
+// those that are touched (null: none is).
+template <int B>
+__device__ __forceinline__ void clear_words(unsigned char* p, long long pitch, int words, const unsigned char* touched, int rows,
+                                            int thread, int threads) {
+  int r = thread / words, c = thread % words;
+  const int rows_on = threads / words, words_on = threads % words;
+  while (r < rows) {
+    if (!touched || !touched[r]) reinterpret_cast<Word<B>*>(p + r * pitch)[c] = Word<B>{};
+    r += rows_on;
+    c += words_on;
+    if (c >= words) {
+      c -= words;
+      ++r;
+    }
+  }
+}
+
+// Rows of `bytes` bytes: by words of 16 bytes where all rows allow them, a warp a row
+// where they do not and are long, else by smaller words.  (39 MB of 320-byte rows: 7 us
+// by words, 19 by a warp a row.)
+__device__ __forceinline__ void clear_rows(unsigned char* p, long long pitch, long long bytes, const unsigned char* touched, int rows,
+                                           int thread, int threads) {
+  const auto all = reinterpret_cast<uintptr_t>(p) | uintptr_t(pitch) | uintptr_t(bytes);
+  if (all % 16 == 0) return clear_words<16>(p, pitch, int(bytes / 16), touched, rows, thread, threads);
+  if (bytes >= 1024) {
+    for (int r = thread / 32; r < rows; r += threads / 32)
+      if (!touched || !touched[r]) clear(p + r * pitch, bytes, thread % 32, 32);
+    return;
+  }
+  if (all % 4 == 0) return clear_words<4>(p, pitch, int(bytes / 4), touched, rows, thread, threads);
+  clear_words<2>(p, pitch, int(bytes / 2), touched, rows, thread, threads);
+}
+
+// Rows that a block of `warps` warps clears: about 64 KiB, less where there are few, and
+// one a warp at least.
+inline int clear_block_rows(long long rows, long long bytes, int warps) {
+  const long long block = std::min<long long>(1 << 16, std::max<long long>(1 << 12, rows * bytes / (4 * device_sms())));
+  return int(std::max<long long>(warps, block / bytes));
+}
+
 // The gradient's rows to be cleared: `rows` stretches of `bytes`, `pitch` bytes apart,
-// by blocks of kSortThreads that take kClearBytes or kSortWarps rows each.
+// by blocks of kSortThreads that take kClearBytes or block_rows rows each.
 struct Clear {
   unsigned char* ptr;
   long long rows, bytes, pitch;
+  int block_rows;
   static constexpr long long kClearBytes = 1 << 18;
   // One stretch where the rows touch.
   __host__ Clear(void* p, long long r, long long b, long long pitch_bytes)
-      : ptr(static_cast<unsigned char*>(p)), rows(pitch_bytes == b ? 1 : r), bytes(pitch_bytes == b ? r * b : b), pitch(pitch_bytes) {}
-  __host__ long long blocks() const { return rows == 1 ? ceil_div_ll(bytes, kClearBytes) : ceil_div_ll(rows, kSortWarps); }
+      : ptr(static_cast<unsigned char*>(p)), rows(pitch_bytes == b ? 1 : r), bytes(pitch_bytes == b ? r * b : b), pitch(pitch_bytes),
+        block_rows(clear_block_rows(r, b, kSortWarps)) {}
+  __host__ long long blocks() const { return rows == 1 ? ceil_div_ll(bytes, kClearBytes) : ceil_div_ll(rows, block_rows); }
   __device__ void run(long long block) const {
     if (rows == 1) {
       const long long begin = block * kClearBytes;
       if (begin < bytes) clear(ptr + begin, min(kClearBytes, bytes - begin), threadIdx.x, kSortThreads);
     } else {
-      const long long r = block * kSortWarps + (threadIdx.x >> 5);
-      if (r < rows) clear(ptr + r * pitch, bytes, threadIdx.x & 31, 32);
+      const long long r = block * block_rows;
+      if (r < rows) clear_rows(ptr + r * pitch, pitch, bytes, nullptr, int(min((long long)block_rows, rows - r)), threadIdx.x, kSortThreads);
     }
   }
 };
@@ -93,16 +136,15 @@ struct Clear {
 struct Rest {
   unsigned char* ptr;
   const unsigned char* touched;
-  long long begin, end, bytes, pitch, block_rows;
-  // By blocks of `warps` warps, each of one row at least and about 64 KiB.
+  long long begin, end, bytes, pitch;
+  int block_rows;
   Rest(unsigned char* p, const unsigned char* t, long long b, long long e, long long row_bytes, long long row_pitch, int warps)
-      : ptr(p), touched(t), begin(b), end(e), bytes(row_bytes), pitch(row_pitch),
-        block_rows(std::max<long long>(warps, (1 << 16) / row_bytes)) {}
+      : ptr(p), touched(t), begin(b), end(e), bytes(row_bytes), pitch(row_pitch), block_rows(clear_block_rows(e - b, row_bytes, warps)) {}
   __host__ long long blocks() const { return ceil_div_ll(end - begin, block_rows); }
   __device__ void run(long long block) const {
-    const long long first = begin + block * block_rows, last = min(end, first + block_rows);
-    for (long long r = first + (threadIdx.x >> 5); r < last; r += blockDim.x >> 5)
-      if (!touched[r]) clear(ptr + r * pitch, bytes, threadIdx.x & 31, 32);
+    const long long r = begin + block * block_rows;
+    if (r < end)
+      clear_rows(ptr + r * pitch, pitch, bytes, touched + r, int(min((long long)block_rows, end - r)), threadIdx.x, blockDim.x);
   }
 };
 
@@ -329,8 +371,7 @@ constexpr int kFewThreads = 256;
 constexpr int kFewEach = kFewTokens / kFewThreads;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kLongRun = 64;         // from here on a block's warps share out the rows, not the columns
-constexpr int kClearRows = 4096;     // rows a clearing block takes at the most,
-constexpr int kClearBytes = 1 << 16; // and about so many bytes
+constexpr int kClearRows = 4096;     // rows a clearing block takes at the most
 
 // The thread's tokens threadIdx.x + k * kFewThreads as rows of the table (-1: none).
 __device__ __forceinline__ void few_tokens(const void* tokens, bool wide, int n, long long rows, long long padding,
@@ -347,7 +388,8 @@ template <typename T, typename O, int N, int W, int S>
 __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ grad, long long grad_stride,
                                                        const void* __restrict__ tokens, bool wide, int n, long long rows,
                                                        long long padding, int width, float scale, bool accumulate,
-                                                       O* __restrict__ out, long long out_stride, int clear_rows, int lanes_log2) {
+                                                       O* __restrict__ out, long long out_stride, int block_rows, int lanes_log2,
+                                                       int parts) {
   __shared__ union {
     struct {
       unsigned short list[kFewTokens];
@@ -358,23 +400,21 @@ __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ gra
   } sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int v[kFewEach];
-  if (int(blockIdx.x) >= n) {
-    const long long first = (long long)(blockIdx.x - n) * clear_rows;
+  if (int(blockIdx.x) >= n * parts) {
+    const long long first = (long long)(blockIdx.x - n * parts) * block_rows;
     few_tokens(tokens, wide, n, rows, padding, v);
-    for (int r = threadIdx.x; r < clear_rows; r += kFewThreads) sh.touched[r] = 0;
+    for (int r = threadIdx.x; r < block_rows; r += kFewThreads) sh.touched[r] = 0;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kFewEach; ++k)
-      if (v[k] >= first && v[k] < first + clear_rows) sh.touched[v[k] - first] = 1;
+      if (v[k] >= first && v[k] < first + block_rows) sh.touched[v[k] - first] = 1;
     __syncthreads();
-    const int lanes = 1 << lanes_log2;
-    for (int r = threadIdx.x >> lanes_log2; r < clear_rows && first + r < rows; r += kFewThreads >> lanes_log2)
-      if (!sh.touched[r])
-        clear(reinterpret_cast<unsigned char*>(out + (first + r) * out_stride), (long long)width * sizeof(O),
-              threadIdx.x & (lanes - 1), lanes);
+    constexpr long long kSize = sizeof(O);
+    clear_rows(reinterpret_cast<unsigned char*>(out + first * out_stride), out_stride * kSize, width * kSize, sh.touched,
+               int(min((long long)block_rows, rows - first)), threadIdx.x, kFewThreads);
     return;
   }
-  const int own = blockIdx.x;
+  const int own = blockIdx.x / parts;
   const long long token = index_at(tokens, wide, own);
   if (token < 0 || token >= rows || token == padding) return;
   few_tokens(tokens, wide, n, rows, padding, v);
@@ -403,10 +443,10 @@ __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ gra
       sh.list[before[k] + __popc(same[k] & ((1u << lane) - 1u))] = (unsigned short)(threadIdx.x + k * kFewThreads);
   __syncthreads();
 
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = 8;
   const int lanes = total > kLongRun ? 32 : 1 << lanes_log2, groups = kFewThreads / lanes;  // threads a row, rows at a time
   const int group = threadIdx.x / lanes, step = word_step<W, S>(lanes);
-  for (int slab = 0; slab < width; slab += lanes * N) {
+  for (int slab = blockIdx.x % parts * lanes * N; slab < width; slab += parts * lanes * N) {
     const int c = slab + first_column<N, W, S>(threadIdx.x & (lanes - 1));
     float acc[N];
 #pragma unroll
@@ -531,11 +571,14 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
       constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;
       O* dst = static_cast<O*>(out.ptr);
       if (few) {
-        const int clear_rows = int(std::min<long long>(kClearRows, std::max<long long>(1, kClearBytes / row_bytes)));
-        const long long blocks = n + (accumulate ? 0 : ceil_div_ll(rows, clear_rows));  // n and blocks are not both 0
+        const int block_rows = std::min(kClearRows, clear_block_rows(rows, row_bytes, kFewWarps));
+        const int lanes_log2 = row_lanes(width, N, 1, std::max(2, decltype(shape)::kLeastLanesLog2), n);
+        // Long rows are shared out among blocks as far as that does not make more than 32 to an SM.
+        const int parts = int(std::max(1LL, std::min<long long>(ceil_div(width, N << lanes_log2), 32LL * device_sms() / std::max(1LL, n))));
+        const long long blocks = n * parts + (accumulate ? 0 : ceil_div_ll(rows, block_rows));  // n and blocks are not both 0
         sum_few<T, O, N, W, S><<<grid_x(blocks), kFewThreads, 0, stream>>>(
             static_cast<const T*>(grad.ptr), grad.stride, tokens.ptr, tokens.wide, int(n), rows, padding, width, scale, accumulate,
-            dst, out.stride, clear_rows, row_lanes(width, N, 1, std::max(2, decltype(shape)::kLeastLanesLog2), n));
+            dst, out.stride, block_rows, lanes_log2, parts);
         PSB_LAUNCH_CHECK();
         return;
       }

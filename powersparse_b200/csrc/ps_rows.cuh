@@ -187,10 +187,12 @@ inline int log2_up(long long v) {
 }
 
 // log2 of the threads that share a row of `width` elements, `n` of them a thread and
-// turn: as many as give a row `turns` turns; fewer where the last turn would leave more
-// than a fifth of the work empty and the `rows` fill the GPU's threads twice over.
+// turn: as many as give a row `turns` turns.  More, while the `rows` leave most of the
+// GPU without threads; fewer where the last turn would leave more than a fifth of the
+// work empty and the rows fill the GPU's threads twice over.
 inline int row_lanes(int width, int n, int turns, int least_log2, long long rows) {
   int lanes = std::min(8, std::max(least_log2, log2_up(ceil_div(ceil_div(width, n), turns))));
+  while (lanes < 8 && rows << lanes < 256LL * device_sms() && n << lanes < width) ++lanes;
   while (lanes > std::max(5, least_log2) && rows << lanes >= 4096LL * device_sms() &&
          (long long)ceil_div(width, n << lanes) * (n << lanes) * 4 > 5LL * width)
     --lanes;
