@@ -408,48 +408,62 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsign
     copy_row<B>(x + t * x_bytes, position + t * top_k, top_k, blanks.rows, words, out, out_bytes, 1 << lanes_log2);
 }
 
-// kSlots rows of a token at a time in registers, added up in the order of the choices.
-// Bound by memory: 8192 tokens of 4096 in 16 bits, 8 experts each and a residual take
-// 112 us, 6.0 TB/s.
-template <typename T, int N, int W, int S, bool kWeighted>
+// A token's rows are added up in the order of the choices, kSlots of them at a time and
+// kTurns stretches of the row, so that a thread has four loads in flight whether a token
+// has many rows or two.  Bound by memory: 8192 tokens of 4096 in 16 bits, 8 experts each
+// and a residual take 108 us, 6.2 TB/s (the positions and weights of a batch are read
+// before its rows: 111 otherwise; eight rows in flight: 112, and 103 against 81 in 32
+// bits, where they cost occupancy).  6799 tokens with 2 experts each: 32 us with (2, 2),
+// 41 with (4, 1).
+template <typename T, int N, int W, int S, bool kWeighted, int kSlots, int kTurns>
 __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict__ y, long long y_stride, long long rows,
                                                             const int* __restrict__ position, const float* __restrict__ weights,
                                                             const T* add, long long add_stride, int tokens, int top_k, int width,
                                                             T* out, long long out_stride, int lanes_log2) {
-  constexpr int kSlots = 4;  // rows in flight
-  const int lanes = 1 << lanes_log2, step = word_step<W, S>(lanes);
+  const int lanes = 1 << lanes_log2, step = word_step<W, S>(lanes), turn = lanes * N;
   const long long t = blockIdx.x * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   if (t >= tokens) return;
-  for (int c = first_column<N, W, S>(threadIdx.x & (lanes - 1)); c < width; c += lanes * N) {
-    float acc[N];
-    Pack<T, N, W> o;
-    o.zero();
-    if (add) o.load_rw(add + t * add_stride, c, step, width);
+  for (int c = first_column<N, W, S>(threadIdx.x & (lanes - 1)); c < width; c += turn * kTurns) {
+    float acc[kTurns][N];
+    Pack<T, N, W> o[kTurns];
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] = o.get(e);
+    for (int k = 0; k < kTurns; ++k) {
+      o[k].zero();
+      if (add) o[k].load_rw(add + t * add_stride, c + k * turn, step, width);
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[k][e] = o[k].get(e);
+    }
     for (int j0 = 0; j0 < top_k; j0 += kSlots) {
-      Pack<T, N, W> v[kSlots];
+      Pack<T, N, W> v[kTurns][kSlots];
       float w[kSlots];
-      bool on[kSlots];
+      int p[kSlots];
 #pragma unroll
       for (int s = 0; s < kSlots; ++s) {
-        const int p = j0 + s < top_k ? position[t * top_k + j0 + s] : -1;
-        on[s] = p >= 0 && p < rows;
-        if (on[s]) {
-          v[s].load(y + p * y_stride, c, step, width);
-          w[s] = kWeighted ? weights[t * top_k + j0 + s] : 1.f;
-        }
+        const bool slot = j0 + s < top_k;
+        p[s] = slot ? position[t * top_k + j0 + s] : -1;
+        w[s] = kWeighted && slot ? weights[t * top_k + j0 + s] : 1.f;
+        if (p[s] >= rows) p[s] = -1;
       }
 #pragma unroll
       for (int s = 0; s < kSlots; ++s)
-        if (on[s]) {
+        if (p[s] >= 0)
 #pragma unroll
-          for (int e = 0; e < N; ++e) acc[e] += w[s] * v[s].get(e);
+          for (int k = 0; k < kTurns; ++k) v[k][s].load(y + p[s] * y_stride, c + k * turn, step, width);
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s)
+        if (p[s] >= 0) {
+#pragma unroll
+          for (int k = 0; k < kTurns; ++k)
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[k][e] += w[s] * v[k][s].get(e);
         }
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) o.set(e, acc[e]);
-    o.store(out + t * out_stride, c, step, width);
+    for (int k = 0; k < kTurns; ++k) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[k].set(e, acc[k][e]);
+      o[k].store(out + t * out_stride, c + k * turn, step, width);
+    }
   }
 }
 
@@ -457,14 +471,15 @@ __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict_
 // each weight on its way out, and with each of its rows of y into a dot product, a warp
 // (or more, for few tokens) a token and kSlots rows in flight.  Bound by memory: 8192
 // tokens of 2048 in 16 bits, 8 experts each, take 101 us, 5.8 TB/s with the rows up to
-// multiples of 128.  Without the bound of 80 registers 104 us.
-template <typename T, int N, int W, int S>
+// multiples of 128.  Without the bound of 80 registers 104 us.  kSlots and kTurns as in
+// combine_rows, by top_k: 6799 tokens of 4096, 2 experts each, take 47 us with (2, 4),
+// 63 with (8, 1).
+template <typename T, int N, int W, int S, int kSlots, int kTurns>
 __global__ void __launch_bounds__(kRowThreads, 3) combine_grad_rows(const T* __restrict__ grad, long long grad_stride, const T* y,
                                                                  long long y_stride, const int* __restrict__ position,
                                                                  Blanks blanks, const float* __restrict__ weights, int tokens,
                                                                  int top_k, int width, T* grad_y, long long grad_y_stride,
                                                                  float* __restrict__ grad_weights, int lanes_log2) {
-  constexpr int kSlots = 8;  // rows in flight, and dot products held
   if (int(blockIdx.x) < blanks.blocks())
     return zero_blanks<W * int(sizeof(T))>(blanks, width / W, reinterpret_cast<unsigned char*>(grad_y),
                                            grad_y_stride * (long long)sizeof(T));
@@ -485,26 +500,32 @@ __global__ void __launch_bounds__(kRowThreads, 3) combine_grad_rows(const T* __r
       dot[s] = 0.f;
     }
     if (live) {
-      for (int c = first_column<N, W, S>(threadIdx.x & (lanes - 1)); c < width; c += lanes * N) {
-        Pack<T, N, W> g, v[kSlots];
-        g.zero();
-        g.load(grad + t * grad_stride, c, step, width);
+      const int turn = lanes * N;
+      for (int c = first_column<N, W, S>(threadIdx.x & (lanes - 1)); c < width; c += turn * kTurns) {
+        Pack<T, N, W> g[kTurns], v[kTurns][kSlots];
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s) {
-          if (N != W) v[s].zero();  // columns behind the row
-          if (p[s] >= 0) v[s].load_rw(y + p[s] * y_stride, c, step, width);
-        }
+        for (int k = 0; k < kTurns; ++k) {
+          g[k].zero();  // columns behind the row
+          g[k].load(grad + t * grad_stride, c + k * turn, step, width);
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s) {
-          if (p[s] < 0) continue;
-          Pack<T, N, W> o;
-#pragma unroll
-          for (int e = 0; e < N; ++e) {
-            dot[s] += g.get(e) * v[s].get(e);
-            o.set(e, w[s] * g.get(e));
+          for (int s = 0; s < kSlots; ++s) {
+            if (N != W || kTurns > 1) v[k][s].zero();
+            if (p[s] >= 0) v[k][s].load_rw(y + p[s] * y_stride, c + k * turn, step, width);
           }
-          o.store(grad_y + p[s] * grad_y_stride, c, step, width);
         }
+#pragma unroll
+        for (int k = 0; k < kTurns; ++k)
+#pragma unroll
+          for (int s = 0; s < kSlots; ++s) {
+            if (p[s] < 0) continue;
+            Pack<T, N, W> o;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              dot[s] += g[k].get(e) * v[k][s].get(e);
+              o.set(e, w[s] * g[k].get(e));
+            }
+            o.store(grad_y + p[s] * grad_y_stride, c + k * turn, step, width);
+          }
       }
     }
 #pragma unroll
@@ -639,10 +660,13 @@ void combine_launch(int dtype, RowsIn y, long long rows, const int* position, co
       constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;
       const int lanes_log2 = row_lanes(width, N, 2, decltype(shape)::kLeastLanesLog2, tokens);
       const unsigned blocks = grid_x(ceil_div_ll(tokens, kRowThreads >> lanes_log2));
-      auto kernel = weights ? combine_rows<T, N, W, S, true> : combine_rows<T, N, W, S, false>;
-      kernel<<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(y.ptr), y.stride, rows, position, weights,
-                                                 static_cast<const T*>(add.ptr), add.stride, tokens, top_k, width,
-                                                 static_cast<T*>(out.ptr), out.stride, lanes_log2);
+      auto run = [&](auto kernel) {
+        kernel<<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(y.ptr), y.stride, rows, position, weights,
+                                                   static_cast<const T*>(add.ptr), add.stride, tokens, top_k, width,
+                                                   static_cast<T*>(out.ptr), out.stride, lanes_log2);
+      };
+      if (top_k > 2) run(weights ? combine_rows<T, N, W, S, true, 4, 1> : combine_rows<T, N, W, S, false, 4, 1>);
+      else run(weights ? combine_rows<T, N, W, S, true, 2, 2> : combine_rows<T, N, W, S, false, 2, 2>);
     });
   });
   PSB_LAUNCH_CHECK();
@@ -663,9 +687,14 @@ void combine_grad_launch(int dtype, RowsIn grad, RowsIn y, long long rows, const
       constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;
       const int lanes_log2 = row_lanes(width, N, 8, 5, tokens);
       const unsigned blocks = grid_x(blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2));
-      combine_grad_rows<T, N, W, S><<<blocks, kRowThreads, 0, stream>>>(
-          static_cast<const T*>(grad.ptr), grad.stride, static_cast<const T*>(y.ptr), y.stride, position, blanks, weights, tokens,
-          top_k, width, static_cast<T*>(grad_y.ptr), grad_y.stride, grad_weights, lanes_log2);
+      auto run = [&](auto kernel) {
+        kernel<<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(grad.ptr), grad.stride, static_cast<const T*>(y.ptr), y.stride,
+                                                   position, blanks, weights, tokens, top_k, width, static_cast<T*>(grad_y.ptr),
+                                                   grad_y.stride, grad_weights, lanes_log2);
+      };
+      if (top_k > 4) run(combine_grad_rows<T, N, W, S, 8, 1>);
+      else if (top_k > 2) run(combine_grad_rows<T, N, W, S, 4, 2>);
+      else run(combine_grad_rows<T, N, W, S, 2, 4>);
     });
   });
   PSB_LAUNCH_CHECK();
