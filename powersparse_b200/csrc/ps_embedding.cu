@@ -481,16 +481,22 @@ __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ gra
 constexpr long long kClearFirst = 96 << 20, kClearLast = 48 << 20;
 
 // Sorted positions a block adds up: more of them make fewer partial rows and joins, but
-// fewer blocks.  64 against 32: 65536 tokens in rows of 1024 64 against 71 us; 16384
-// tokens in rows of 2048 188 against 180.
-int chunk_of(long long n) { return n >= 32768 ? 64 : n >= 16384 ? 32 : 16; }
+// fewer threads; where rows are narrow there are few threads a block, and the blocks
+// become smaller until the GPU is about a third full.  64 against 32: 65536 tokens in
+// rows of 1024 64 against 71 us; 16384 tokens in rows of 2048 188 against 180.
+int chunk_of(long long n, int width) {
+  int chunk = n >= 32768 ? 64 : n >= 16384 ? 32 : 16;
+  const long long threads = ceil_div(width, 8 * 32) * 32;
+  while (chunk > 8 && ceil_div_ll(n, chunk) * threads < 65536) chunk /= 2;
+  return chunk;
+}
 
 constexpr size_t align_up(size_t v) { return (v + 255) / 256 * 256; }
 
 struct Workspace {
   size_t a, b, join_count, shorter, longer, touched, partial, bytes;
   Workspace(long long n, long long rows, int width) {
-    const long long chunks = ceil_div_ll(n, chunk_of(n));
+    const long long chunks = ceil_div_ll(n, chunk_of(n, width));
     a = 0;
     b = a + align_up(size_t(n) * sizeof(Item));
     join_count = b + align_up(size_t(n) * sizeof(Item));
@@ -532,7 +538,7 @@ size_t embedding_grad_workspace(long long tokens, long long rows, int width) {
 void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float scale, long long padding, bool accumulate,
                            int out_dtype, RowsOut out, long long rows, int width, void* workspace, cudaStream_t stream) {
   const long long n = tokens.count;
-  const int in_size = dtype_size(grad_dtype), out_size = dtype_size(out_dtype), chunk = chunk_of(n);
+  const int in_size = dtype_size(grad_dtype), out_size = dtype_size(out_dtype), chunk = chunk_of(n, width);
   if (n == 0 && accumulate) return;
   const Workspace at(n, rows, width);
   char* ws = static_cast<char*>(workspace);

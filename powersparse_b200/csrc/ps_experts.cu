@@ -467,15 +467,38 @@ __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict_
   }
 }
 
+// Sums of K numbers each over a warp: a lane gets that of number lane / (32 / K).  While
+// there is more than one number left, half the lanes go on with one half of them and half
+// with the other, so eight sums take 9 shuffles, not 40.
+template <int K>
+__device__ __forceinline__ float sum_slots(float (&d)[K]) {
+  const int lane = threadIdx.x & 31;
+  int far = 16;
+#pragma unroll
+  for (int n = K / 2; n > 0; n /= 2, far /= 2) {
+    const bool upper = lane & far;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = upper ? d[i + n] : d[i], send = upper ? d[i] : d[i + n];
+      d[i] = keep + __shfl_xor_sync(0xffffffffu, send, far);
+    }
+  }
+  float v = d[0];
+#pragma unroll
+  for (; far > 0; far /= 2) v += __shfl_xor_sync(0xffffffffu, v, far);
+  return v;
+}
+
 // Both gradients in one pass: the token's gradient row is read once and multiplied with
 // each weight on its way out, and with each of its rows of y into a dot product, a warp
-// (or more, for few tokens) a token and kSlots rows in flight.  Bound by memory: 8192
-// tokens of 2048 in 16 bits, 8 experts each, take 101 us, 5.8 TB/s with the rows up to
-// multiples of 128.  Without the bound of 80 registers 104 us.  kSlots and kTurns as in
-// combine_rows, by top_k: 6799 tokens of 4096, 2 experts each, take 47 us with (2, 4),
-// 63 with (8, 1).
+// (or more, for few tokens) a token, kSlots rows and kTurns stretches of them in flight.
+// Bound by memory: 8192 tokens of 2048 in 16 bits, 8 experts each, take 100 us, 5.8 TB/s
+// with the rows up to multiples of 128 (104 without the bound of 80 registers); 6799
+// tokens of 4096, 2 experts each, 47 us with (2, 4), 63 with (8, 1).  Ragged rows are
+// bound by latency and want more warps instead: 15687 tokens of 1893, one expert each,
+// 57 us with (2, 2) in 64 registers, 102 with (2, 4) in 128.
 template <typename T, int N, int W, int S, int kSlots, int kTurns>
-__global__ void __launch_bounds__(kRowThreads, 3) combine_grad_rows(const T* __restrict__ grad, long long grad_stride, const T* y,
+__global__ void __launch_bounds__(kRowThreads, W == N ? 3 : 4) combine_grad_rows(const T* __restrict__ grad, long long grad_stride, const T* y,
                                                                  long long y_stride, const int* __restrict__ position,
                                                                  Blanks blanks, const float* __restrict__ weights, int tokens,
                                                                  int top_k, int width, T* grad_y, long long grad_y_stride,
@@ -528,23 +551,20 @@ __global__ void __launch_bounds__(kRowThreads, 3) combine_grad_rows(const T* __r
           }
       }
     }
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s) dot[s] = warp_sum(dot[s]);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = lanes >> 5;
+    const float dot_warp = sum_slots<kSlots>(dot);
+    constexpr int kEach = 32 / kSlots;  // lanes that end up with a slot's sum
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = lanes >> 5, slot = lane / kEach;
     if (warps > 1) {
       __syncthreads();
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s)
-        if (lane == s) parts[warp][s] = dot[s];
+      if (lane % kEach == 0) parts[warp][slot] = dot_warp;
       __syncthreads();
     }
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s)
-      if (lane == s && live && j0 + s < top_k && warp % warps == 0) {
-        float sum = dot[s];
-        for (int k = 1; k < warps; ++k) sum += parts[warp + k][s];
-        grad_weights[t * top_k + j0 + s] = p[s] >= 0 ? sum : 0.f;
-      }
+    if (lane % kEach == 0 && live && j0 + slot < top_k && warp % warps == 0) {
+      float sum = dot_warp;
+      for (int k = 1; k < warps; ++k) sum += parts[warp + k][slot];
+      const int at = position[t * top_k + j0 + slot];
+      grad_weights[t * top_k + j0 + slot] = at >= 0 && at < rows ? sum : 0.f;
+    }
   }
 }
 
@@ -692,9 +712,14 @@ void combine_grad_launch(int dtype, RowsIn grad, RowsIn y, long long rows, const
                                                    position, blanks, weights, tokens, top_k, width, static_cast<T*>(grad_y.ptr),
                                                    grad_y.stride, grad_weights, lanes_log2);
       };
-      if (top_k > 4) run(combine_grad_rows<T, N, W, S, 8, 1>);
-      else if (top_k > 2) run(combine_grad_rows<T, N, W, S, 4, 2>);
-      else run(combine_grad_rows<T, N, W, S, 2, 4>);
+      if constexpr (W == N) {
+        if (top_k > 4) run(combine_grad_rows<T, N, W, S, 8, 1>);
+        else if (top_k > 2) run(combine_grad_rows<T, N, W, S, 4, 2>);
+        else run(combine_grad_rows<T, N, W, S, 2, 4>);
+      } else {
+        if (top_k > 2) run(combine_grad_rows<T, N, W, S, 4, 1>);
+        else run(combine_grad_rows<T, N, W, S, 2, 2>);
+      }
     });
   });
   PSB_LAUNCH_CHECK();

@@ -169,16 +169,16 @@ def test_embedding_grad_order_of_large_batches(kind, n, rows):
     assert torch.equal(got, psb.embedding_grad(grad, tokens, rows, dtype=F32))  # the same bits again
 
 
-@pytest.mark.parametrize("n,chunk", [(2100, 16), (20000, 32)])
+@pytest.mark.parametrize("n,width", [(2100, 40), (20000, 40), (20000, 1032), (40000, 1032)])
 @pytest.mark.parametrize("lengths", [(1, 15, 16, 17), (16, 32, 48), (31, 33, 1), (30, 2, 32, 1), (47, 17, 1), (64, 63, 65, 1), (200, 5), (33,)])
-def test_embedding_grad_of_runs_about_the_chunks_borders(n, chunk, lengths):
-    """Runs of every length about one, two and more chunks of the sorted batch, begun at every place in a chunk."""
+def test_embedding_grad_of_runs_about_the_chunks_borders(n, width, lengths):
+    """Runs of every length about one, two and more chunks (of 8 to 64) of the sorted batch, begun at every place in one."""
     g = gen(n)
     runs = torch.tensor(lengths * (n // sum(lengths) + 1), device="cuda")
     tokens = torch.repeat_interleave(torch.arange(len(runs), device="cuda"), runs)[:n]
     tokens = tokens[torch.randperm(n, generator=g, device="cuda")]
     tokens = torch.where(tokens % 5 == 4, tokens + len(runs), tokens)  # some outside
-    grad = randn(g, n, 40, dtype=BF16)
+    grad = randn(g, n, width, dtype=BF16)
     want, slack = grad64(grad, tokens, len(runs), 1.0)
     check(psb.embedding_grad(grad, tokens, len(runs), dtype=F32), want, slack)
 
