@@ -225,13 +225,14 @@ __device__ __forceinline__ void write_sum(O* row, int c, int step, int width, co
 }
 
 template <typename T, typename O, int N, int W>
-__global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ grad, long long grad_stride,
+__global__ void __launch_bounds__(kSumThreads, 8) sum_runs(const T* __restrict__ grad, long long grad_stride,
                                                         const Item* items, long long n, uint32_t rows, int width, float scale, bool accumulate,
                                                         O* __restrict__ out, long long out_stride, int chunk,
                                                         float* __restrict__ partial, Joins joins, int sum_blocks, int slabs, Rest rest) {
   constexpr int kUnroll = 8;
   constexpr uint32_t kNone = 0xffffffffu;
   __shared__ uint32_t key[kMaxChunk + 2], at[kMaxChunk];
+  static_assert(kMaxChunk % 32 == 0 && kMaxChunk <= 64);
   let_next_start();
   wait_for_previous();
   if (int(blockIdx.x) >= sum_blocks) return rest.run(blockIdx.x - sum_blocks);
@@ -252,29 +253,40 @@ __global__ void __launch_bounds__(kSumThreads) sum_runs(const T* __restrict__ gr
       (longer ? joins.longer : joins.shorter)[atomicAdd(joins.count + longer, 1)] = {token, uint32_t(block)};
     }
   }
+  // Where runs end in the chunk, as bits, and how many of its positions name a row (the
+  // empty places are sorted behind them): all that the loop asks for each position.
+  const int lane = threadIdx.x & 31;
+  unsigned long long ends = 0;
+  int total = 0;
+#pragma unroll
+  for (int half = 0; half < kMaxChunk / 32; ++half) {
+    const int i = half * 32 + lane;
+    const bool on = i < count && key[i + 1] < rows;
+    ends |= (unsigned long long)__ballot_sync(0xffffffffu, on && (key[i + 1] != key[i + 2] || i + 1 == count)) << (half * 32);
+    total += __popc(__ballot_sync(0xffffffffu, on));
+  }
   constexpr int step = 32 * W;
   const int c = first_column<N, W, 32>(blockIdx.x % slabs * blockDim.x + threadIdx.x);
   if (c >= width) return;
+  const bool goes_on = key[count] == key[count + 1];
+  bool before = key[0] == key[1];  // the current run began before the chunk
   float acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
-  bool before = key[0] == key[1];  // the current run began before the chunk
-  for (int i = 0; i < count; i += kUnroll) {
+  for (int i = 0; i < total; i += kUnroll) {
     Pack<T, N, W> v[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
-      if (i + u < count && key[i + u + 1] < rows) v[u].load(grad + (long long)at[i + u] * grad_stride, c, step, width);
+      v[u].load(grad + (long long)at[min(i + u, total - 1)] * grad_stride, c, step, width);
+    const unsigned here = unsigned(ends >> i) & ((1u << kUnroll) - 1u);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (i + u >= count) break;
-      const uint32_t k = key[i + u + 1];
-      if (k >= rows) return;  // sorted: nothing but empty places from here on
+      if (i + u >= total) break;
 #pragma unroll
       for (int e = 0; e < N; ++e) acc[e] += v[u].get(e);
-      if (key[i + u + 2] == k && i + u + 1 < count) continue;
-      const bool after = key[i + u + 2] == k;
-      if (!before && !after) {
-        write_sum<O, N, W>(out + (long long)k * out_stride, c, step, width, acc, scale, accumulate);
+      if (!(here >> u & 1)) continue;
+      if (!before && !(goes_on && i + u + 1 == count)) {
+        write_sum<O, N, W>(out + (long long)key[i + u + 1] * out_stride, c, step, width, acc, scale, accumulate);
       } else {
         Pack<float, N, W> sum;
 #pragma unroll

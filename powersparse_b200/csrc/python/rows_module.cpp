@@ -5,7 +5,7 @@
 // addresses that bind() was given, so that it serves whichever library the package has
 // loaded.  Native because at a serving step's sizes the kernels take a few
 // microseconds, and the same checks in Python with a ctypes call took 14 (24 for
-// dispatch, with its four outputs) against the kernels' 2 to 5.
+// dispatch, with its four outputs) against the kernels' 2 to 5; these take 5 (7).
 //
 // Every function takes positional arguments only, checked for their number; rows.py
 // holds the signatures.  ValueError for refused arguments, RuntimeError for CUDA errors.
@@ -125,6 +125,7 @@ Matrix matrix_like(PyObject* o, const char* name, c10::Device device, at::Scalar
   require_device(t, name, device);
   Matrix m = matrix_of(t, name);
   if (t.scalar_type() != type) refuse(std::string(name) + " must be " + text(type) + ", not " + text(t.scalar_type()));
+  if (rows < 0 && m.width != width) refuse(std::string(name) + " must have rows of " + std::to_string(width) + " elements");
   if ((rows >= 0 && m.rows != rows) || m.width != width)
     refuse(std::string(name) + " must have the shape " + text({rows, width}) + ", not " + text(t.sizes()));
   return m;

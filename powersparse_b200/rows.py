@@ -58,7 +58,16 @@ def _load_native():
     return module
 
 
-_native = _load_native()
+class _Unloaded:
+    """Stands for the native module until its first use."""
+
+    def __getattr__(self, name):
+        global _native
+        _native = _load_native()
+        return getattr(_native, name)
+
+
+_native = _Unloaded()
 
 
 def _handle(stream, tensor):
