@@ -208,9 +208,10 @@ struct Joins {
 
 // Bound by memory where the rows are wide and the table large (16384 tokens of 2048 in
 // 16 bits into 131072 rows in 32: 176 us for sort, sums, joins and clearing together, 98%
-// of the copy rate).  Ragged rows (50003 of 515 in 16 bits, 43 us in all) are bound by
-// latency and instructions: 21 us for the sort's two passes, about 14 for the sums, 8
-// for the joins.
+// of the copy rate).  Ragged rows (50003 of 515 in 16 bits, 40 us in all) are bound by
+// latency and instructions: 21 us for the sort's two passes, about 11 for the sums, 8
+// for the joins.  Eight rows in flight and eight blocks an SM: sixteen rows or ten blocks
+// took 2 and 6 us longer there.
 constexpr int kSumThreads = 128;
 constexpr int kMaxChunk = 64;
 
