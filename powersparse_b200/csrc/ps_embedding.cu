@@ -226,10 +226,11 @@ __device__ __forceinline__ void write_sum(O* row, int c, int step, int width, co
 }
 
 template <typename T, typename O, int N, int W>
-__global__ void __launch_bounds__(kSumThreads, 8) sum_runs(const T* __restrict__ grad, long long grad_stride,
-                                                        const Item* items, long long n, uint32_t rows, int width, float scale, bool accumulate,
-                                                        O* __restrict__ out, long long out_stride, int chunk,
-                                                        float* __restrict__ partial, Joins joins, int sum_blocks, int slabs, Rest rest) {
+__global__ void __launch_bounds__(kSumThreads, 8) sum_runs(const T* __restrict__ grad, long long grad_stride, const Item* items,
+                                                           long long n, uint32_t rows, int width, float scale, bool accumulate,
+                                                           O* __restrict__ out, long long out_stride, int chunk,
+                                                           float* __restrict__ partial, Joins joins, int sum_blocks, int slabs,
+                                                           Rest rest) {
   constexpr int kUnroll = 8;
   constexpr uint32_t kNone = 0xffffffffu;
   __shared__ uint32_t key[kMaxChunk + 2], at[kMaxChunk];

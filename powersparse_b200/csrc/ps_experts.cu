@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const floa
   float* own = spread[warp];
 #pragma unroll
   for (int v = 0; v < V; ++v) own[v * 32 + lane] = 0.f;
+  __syncwarp();
   const float inner = warp_sum(g * w);
   float value = kNormalize ? w * (g - inner) : g;
   const unsigned same = __match_any_sync(0xffffffffu, mine);

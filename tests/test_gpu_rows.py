@@ -157,7 +157,8 @@ def test_embedding_grad(dtype, out, width):
 
 
 @pytest.mark.parametrize("kind", ["any", "skewed", "one", "distinct", "sorted", "empty"])
-@pytest.mark.parametrize("n,rows", [(31, 9), (65, 5000), (2047, 300), (2048, 40000), (20000, 40000), (70001, 70001), (16384, 1025), (40000, 3_000_000), (9000, 512), (2049, 1023)])
+@pytest.mark.parametrize("n,rows", [(31, 9), (65, 5000), (2047, 300), (2048, 40000), (20000, 40000), (70001, 70001),
+                                    (16384, 1025), (40000, 3_000_000), (9000, 512), (2049, 1023), (131072, 700_000), (131073, 1_000_000)])
 def test_embedding_grad_order_of_large_batches(kind, n, rows):
     g = gen(n + rows)
     if kind == "distinct" and n > rows:
@@ -358,6 +359,21 @@ def test_route_with_nan_and_inf():
         grad[3, 2:] = math.nan  # beside a choice of -1: not used
         got = psb.route_grad(grad, logits, weights, chosen, normalize)
         assert got[3:].isfinite().all() and got[0].isnan().any()
+
+
+def test_route_gradient_with_a_choice_that_stands_twice():
+    """route never gives one, but a caller may: the gradients of both places add up, as the formula says."""
+    logits = randn(gen(8), 3, 40)
+    chosen = torch.tensor([[5, 5, 7], [1, 0, 1], [9, 9, 9]], dtype=torch.int32, device="cuda")
+    weights, grad = torch.rand(3, 3, generator=gen(9), device="cuda"), randn(gen(10), 3, 3)
+    p = torch.softmax(logits.double(), 1)
+    inner = (grad.double() * weights.double()).sum(1, keepdim=True)
+    dense = torch.zeros_like(p).scatter_add_(1, chosen.long(), grad.double())
+    size = grad.double().abs().sum(1, keepdim=True) * 2
+    check(psb.route_grad(grad, logits, weights, chosen, False), p * (dense - inner), p * size * (softmax_slack(logits) + 8 * U))
+    share = weights.double() * (grad.double() - inner)
+    want = torch.zeros_like(p).scatter_add_(1, chosen.long(), share)
+    check(psb.route_grad(grad, logits, weights, chosen, True), want, size * 8 * U)
 
 
 def test_route_gradient_against_differences():
