@@ -22,10 +22,11 @@ constexpr int kRowThreads = 256;
 constexpr int kRowUnroll = 4;
 
 template <typename T, int N, int W, int S>
-__global__ void __launch_bounds__(kRowThreads) embedding_rows(const T* __restrict__ table, long long table_stride, long long rows,
-                                                              const void* __restrict__ tokens, bool wide, long long n, int width,
-                                                              float scale, T* __restrict__ out, long long out_stride,
+__global__ void __launch_bounds__(kRowThreads) embedding_rows(const T* table, long long table_stride, long long rows,
+                                                              const void* tokens, bool wide, long long n, int width,
+                                                              float scale, T* out, long long out_stride,
                                                               int lanes_log2) {
+  wait_for_previous();
   const int lanes = 1 << lanes_log2, step = word_step<W, S>(lanes);
   const long long i = blockIdx.x * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   if (i >= n) return;
@@ -154,7 +155,7 @@ struct Rest {
 // names need it, and what the others cost is hidden, since the sort leaves most of the
 // GPU idle.  touched (null unless rows are left to the later kernels): 1 for every token
 // that occurs.  counts: two numbers to be set to zero.
-__global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __restrict__ tokens, bool wide, long long n,
+__global__ void __launch_bounds__(kSortThreads) embedding_order(const void* tokens, bool wide, long long n,
                                                                 long long rows, long long padding, int pass_bits, int passes,
                                                                 Item* a, Item* b, int* counts, unsigned char* touched,
                                                                 Clear zeros) {
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_order(const void* __re
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   let_next_start();
+  wait_for_previous();
   if (int(blockIdx.x) >= blocks) return zeros.run(blockIdx.x - blocks);
   const int digits = 1 << pass_bits;
   const SortShared sh(smem, digits);
@@ -219,17 +221,17 @@ template <typename O, int N, int W>
 __device__ __forceinline__ void write_sum(O* row, int c, int step, int width, const float (&acc)[N], float scale, bool accumulate) {
   Pack<O, N, W> v;
   v.zero();
-  if (accumulate) v.load_rw(row, c, step, width);
+  if (accumulate) v.load(row, c, step, width);
 #pragma unroll
   for (int e = 0; e < N; ++e) v.set(e, accumulate ? v.get(e) + acc[e] * scale : acc[e] * scale);
   v.store(row, c, step, width);
 }
 
 template <typename T, typename O, int N, int W>
-__global__ void __launch_bounds__(kSumThreads, 8) sum_runs(const T* __restrict__ grad, long long grad_stride, const Item* items,
+__global__ void __launch_bounds__(kSumThreads, 8) sum_runs(const T* grad, long long grad_stride, const Item* items,
                                                            long long n, uint32_t rows, int width, float scale, bool accumulate,
-                                                           O* __restrict__ out, long long out_stride, int chunk,
-                                                           float* __restrict__ partial, Joins joins, int sum_blocks, int slabs,
+                                                           O* out, long long out_stride, int chunk,
+                                                           float* partial, Joins joins, int sum_blocks, int slabs,
                                                            Rest rest) {
   constexpr int kUnroll = 8;
   constexpr uint32_t kNone = 0xffffffffu;
@@ -309,7 +311,7 @@ constexpr int kJoinWarps = 16;
 
 template <typename O, int N, int W>
 __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, long long n, int width, float scale,
-                                                             bool accumulate, O* __restrict__ out, long long out_stride, int chunk,
+                                                             bool accumulate, O* out, long long out_stride, int chunk,
                                                              const float* partial, Joins joins, int chunks, int long_blocks,
                                                              int short_blocks, int slabs, Rest rest) {
   constexpr int kUnroll = kShortRun;
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, 
       const long long j = own + first + u * stride;
       const bool inside = j * chunk < n;
       v[u].zero();
-      if (inside) v[u].load_rw(partial + (j * 2 + (j == own ? 1 : 0)) * width, c, 32 * W, width);
+      if (inside) v[u].load(partial + (j * 2 + (j == own ? 1 : 0)) * width, c, 32 * W, width);
       on[u] = j == own || (inside && items[j * chunk].token == join.token);
     }
 #pragma unroll
@@ -399,10 +401,10 @@ __device__ __forceinline__ void few_tokens(const void* tokens, bool wide, int n,
 }
 
 template <typename T, typename O, int N, int W, int S>
-__global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ grad, long long grad_stride,
-                                                       const void* __restrict__ tokens, bool wide, int n, long long rows,
+__global__ void __launch_bounds__(kFewThreads) sum_few(const T* grad, long long grad_stride,
+                                                       const void* tokens, bool wide, int n, long long rows,
                                                        long long padding, int width, float scale, bool accumulate,
-                                                       O* __restrict__ out, long long out_stride, int block_rows, int lanes_log2,
+                                                       O* out, long long out_stride, int block_rows, int lanes_log2,
                                                        int parts) {
   __shared__ union {
     struct {
@@ -413,6 +415,7 @@ __global__ void __launch_bounds__(kFewThreads) sum_few(const T* __restrict__ gra
     unsigned char touched[kClearRows];
   } sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  wait_for_previous();
   int v[kFewEach];
   if (int(blockIdx.x) >= n * parts) {
     const long long first = (long long)(blockIdx.x - n * parts) * block_rows;
@@ -537,12 +540,10 @@ void embedding_launch(int dtype, RowsIn table, long long rows, int width, Indice
       constexpr int N = decltype(shape)::N, W = decltype(shape)::W, S = decltype(shape)::S;
       const int lanes_log2 = row_lanes(width, N * kRowUnroll, 1, decltype(shape)::kLeastLanesLog2, tokens.count);
       const unsigned blocks = grid_x(ceil_div_ll(tokens.count, kRowThreads >> lanes_log2));
-      embedding_rows<T, N, W, S><<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(table.ptr), table.stride, rows, tokens.ptr,
-                                                                  tokens.wide, tokens.count, width, scale,
-                                                                  static_cast<T*>(out.ptr), out.stride, lanes_log2);
+      launch_after(embedding_rows<T, N, W, S>, blocks, kRowThreads, stream, static_cast<const T*>(table.ptr), table.stride, rows,
+                   tokens.ptr, tokens.wide, tokens.count, width, scale, static_cast<T*>(out.ptr), out.stride, lanes_log2);
     });
   });
-  PSB_LAUNCH_CHECK();
 }
 
 size_t embedding_grad_workspace(long long tokens, long long rows, int width) {
@@ -596,10 +597,9 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
         // Long rows are shared out among blocks as far as that does not make more than 32 to an SM.
         const int parts = int(std::max(1LL, std::min<long long>(ceil_div(width, N << lanes_log2), 32LL * device_sms() / std::max(1LL, n))));
         const long long blocks = n * parts + (accumulate ? 0 : ceil_div_ll(rows, block_rows));  // n and blocks are not both 0
-        sum_few<T, O, N, W, S><<<grid_x(blocks), kFewThreads, 0, stream>>>(
-            static_cast<const T*>(grad.ptr), grad.stride, tokens.ptr, tokens.wide, int(n), rows, padding, width, scale, accumulate,
-            dst, out.stride, block_rows, lanes_log2, parts);
-        PSB_LAUNCH_CHECK();
+        launch_after(sum_few<T, O, N, W, S>, grid_x(blocks), kFewThreads, stream, static_cast<const T*>(grad.ptr), grad.stride,
+                     tokens.ptr, tokens.wide, int(n), rows, padding, width, scale, accumulate, dst, out.stride, block_rows, lanes_log2,
+                     parts);
         return;
       }
       const int chunks = int(ceil_div_ll(n, chunk));

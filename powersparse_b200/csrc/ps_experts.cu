@@ -133,12 +133,13 @@ __device__ __forceinline__ int top_scores(float (&x)[V], int top_k, Gathered& g,
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* __restrict__ logits, long long stride, bool words,
+__global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* logits, long long stride, bool words,
                                                                  int tokens, int experts, int top_k, bool normalize,
-                                                                 float* __restrict__ weights, int* __restrict__ chosen) {
+                                                                 float* weights, int* chosen) {
   __shared__ __align__(16) Gathered gathered[kRouteWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long t = blockIdx.x * (long long)kRouteWarps + warp;
+  wait_for_previous();
   if (t >= tokens) return;
   float x[V], top;
   bool nan = false;
@@ -181,14 +182,15 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* __rest
 // words apart, so that a warp writes whole sectors.  16384 tokens of 256 experts in FP32:
 // 7.8 us, 4.5 TB/s, where handing each choice round the warp took 9.3.
 template <typename T, int V, bool kNormalize>
-__global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const float* __restrict__ grad, const T* __restrict__ logits,
-                                                                      long long stride, bool words, const float* __restrict__ weights,
-                                                                      const int* __restrict__ chosen, int tokens, int experts,
-                                                                      int top_k, T* __restrict__ out, long long out_stride) {
+__global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const float* grad, const T* logits,
+                                                                      long long stride, bool words, const float* weights,
+                                                                      const int* chosen, int tokens, int experts,
+                                                                      int top_k, T* out, long long out_stride) {
   constexpr int W = kScoreWord<T, V>;
   __shared__ __align__(16) float spread[kRouteWarps][32 * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long t = blockIdx.x * (long long)kRouteWarps + warp;
+  wait_for_previous();
   if (t >= tokens) return;
   Pack<T, V, W> x;
   if (!kNormalize) load_scores<T, V>(x, logits + t * stride, lane * W, 32 * W, experts, words);
@@ -238,14 +240,15 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const floa
 }
 
 // ---- order of the slots by expert ---------------------------------------------------
-__global__ void __launch_bounds__(kSortThreads) expert_order(const void* __restrict__ chosen, bool wide, long long n, int experts,
-                                                             int align, int* __restrict__ position, int* __restrict__ offsets,
-                                                             int* __restrict__ counts) {
+__global__ void __launch_bounds__(kSortThreads) expert_order(const void* chosen, bool wide, long long n, int experts,
+                                                             int align, int* position, int* offsets,
+                                                             int* counts) {
   extern __shared__ __align__(16) unsigned char smem[];
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   let_next_start();
+  wait_for_previous();
   auto expert = [&](long long i) {
     const long long e = index_at(chosen, wide, i);
     return e >= 0 && e < experts ? int(e) : -1;
@@ -312,7 +315,7 @@ __device__ __forceinline__ void copy_row(const unsigned char* x, const int* posi
     Word<B> v[kRowUnroll];
 #pragma unroll
     for (int u = 0; u < kRowUnroll; ++u)
-      if (c + u * lanes < words) v[u] = __ldg(src + c + u * lanes);
+      if (c + u * lanes < words) v[u] = src[c + u * lanes];
     for (int j = 0; j < top_k; ++j) {
       const int p = position[j];
       if (p < 0 || p >= rows) continue;
@@ -331,14 +334,15 @@ __device__ __forceinline__ void copy_row(const unsigned char* x, const int* posi
 constexpr int kFewSlots = 2048;
 
 template <int B>
-__global__ void __launch_bounds__(kRowThreads) dispatch_few(const unsigned char* __restrict__ x, long long x_bytes,
-                                                            const void* __restrict__ chosen, bool wide, int n, int align,
-                                                            int* __restrict__ position, int* __restrict__ offsets,
-                                                            int* __restrict__ counts, Blanks blanks, int top_k, int words,
-                                                            unsigned char* __restrict__ out, long long out_bytes) {
+__global__ void __launch_bounds__(kRowThreads) dispatch_few(const unsigned char* x, long long x_bytes,
+                                                            const void* chosen, bool wide, int n, int align,
+                                                            int* position, int* offsets,
+                                                            int* counts, Blanks blanks, int top_k, int words,
+                                                            unsigned char* out, long long out_bytes) {
   __shared__ int expert[kFewSlots], count[kMaxExperts], begin[kMaxExperts + 1], place[kMaxTopK];
   __shared__ int warp_total[kRowThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, experts = blanks.experts;
+  wait_for_previous();
   for (int e = threadIdx.x; e < experts; e += kRowThreads) count[e] = 0;
   __syncthreads();
   for (int s = threadIdx.x; s < n; s += kRowThreads) {
@@ -398,9 +402,9 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_few(const unsigned char*
 }
 
 template <int B>
-__global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsigned char* __restrict__ x, long long x_bytes,
+__global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsigned char* x, long long x_bytes,
                                                                     const int* position, Blanks blanks, int tokens, int top_k,
-                                                                    int words, unsigned char* __restrict__ out,
+                                                                    int words, unsigned char* out,
                                                                     long long out_bytes, int lanes_log2) {
   wait_for_previous();
   if (int(blockIdx.x) < blanks.blocks()) return zero_blanks<B>(blanks, words, out, out_bytes);
@@ -417,10 +421,11 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsign
 // bits, where they cost occupancy).  6799 tokens with 2 experts each: 32 us with (2, 2),
 // 41 with (4, 1).
 template <typename T, int N, int W, int S, bool kWeighted, int kSlots, int kTurns>
-__global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict__ y, long long y_stride, long long rows,
-                                                            const int* __restrict__ position, const float* __restrict__ weights,
+__global__ void __launch_bounds__(kRowThreads) combine_rows(const T* y, long long y_stride, long long rows,
+                                                            const int* position, const float* weights,
                                                             const T* add, long long add_stride, int tokens, int top_k, int width,
                                                             T* out, long long out_stride, int lanes_log2) {
+  wait_for_previous();
   const int lanes = 1 << lanes_log2, step = word_step<W, S>(lanes), turn = lanes * N;
   const long long t = blockIdx.x * (long long)(kRowThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
   if (t >= tokens) return;
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* __restrict_
 #pragma unroll
     for (int k = 0; k < kTurns; ++k) {
       o[k].zero();
-      if (add) o[k].load_rw(add + t * add_stride, c + k * turn, step, width);
+      if (add) o[k].load(add + t * add_stride, c + k * turn, step, width);
 #pragma unroll
       for (int e = 0; e < N; ++e) acc[k][e] = o[k].get(e);
     }
@@ -499,11 +504,12 @@ __device__ __forceinline__ float sum_slots(float (&d)[K]) {
 // bound by latency and want more warps instead: 15687 tokens of 1893, one expert each,
 // 57 us with (2, 2) in 64 registers, 102 with (2, 4) in 128.
 template <typename T, int N, int W, int S, int kSlots, int kTurns>
-__global__ void __launch_bounds__(kRowThreads, W == N ? 3 : 4) combine_grad_rows(const T* __restrict__ grad, long long grad_stride, const T* y,
-                                                                 long long y_stride, const int* __restrict__ position,
-                                                                 Blanks blanks, const float* __restrict__ weights, int tokens,
+__global__ void __launch_bounds__(kRowThreads, W == N ? 3 : 4) combine_grad_rows(const T* grad, long long grad_stride, const T* y,
+                                                                 long long y_stride, const int* position,
+                                                                 Blanks blanks, const float* weights, int tokens,
                                                                  int top_k, int width, T* grad_y, long long grad_y_stride,
-                                                                 float* __restrict__ grad_weights, int lanes_log2) {
+                                                                 float* grad_weights, int lanes_log2) {
+  wait_for_previous();
   if (int(blockIdx.x) < blanks.blocks())
     return zero_blanks<W * int(sizeof(T))>(blanks, width / W, reinterpret_cast<unsigned char*>(grad_y),
                                            grad_y_stride * (long long)sizeof(T));
@@ -534,7 +540,7 @@ __global__ void __launch_bounds__(kRowThreads, W == N ? 3 : 4) combine_grad_rows
 #pragma unroll
           for (int s = 0; s < kSlots; ++s) {
             if (N != W || kTurns > 1) v[k][s].zero();
-            if (p[s] >= 0) v[k][s].load_rw(y + p[s] * y_stride, c + k * turn, step, width);
+            if (p[s] >= 0) v[k][s].load(y + p[s] * y_stride, c + k * turn, step, width);
           }
         }
 #pragma unroll
@@ -604,11 +610,10 @@ void route_launch(int dtype, RowsIn logits, int tokens, int experts, int top_k, 
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
     with_scores<T>(experts, fits, [&](auto v, bool words) {
-      route_tokens<T, decltype(v)::value><<<ceil_div(tokens, kRouteWarps), kRouteWarps * 32, 0, stream>>>(
-          static_cast<const T*>(logits.ptr), logits.stride, words, tokens, experts, top_k, normalize, weights, chosen);
+      launch_after(route_tokens<T, decltype(v)::value>, ceil_div(tokens, kRouteWarps), kRouteWarps * 32, stream,
+                   static_cast<const T*>(logits.ptr), logits.stride, words, tokens, experts, top_k, normalize, weights, chosen);
     });
   });
-  PSB_LAUNCH_CHECK();
 }
 
 void route_grad_launch(int dtype, const float* grad_weights, RowsIn logits, const float* weights, const int* chosen, int tokens,
@@ -623,12 +628,11 @@ void route_grad_launch(int dtype, const float* grad_weights, RowsIn logits, cons
     with_scores<T>(experts, fits, [&](auto v, bool words) {
       constexpr int V = decltype(v)::value;
       auto kernel = normalize ? route_grad_tokens<T, V, true> : route_grad_tokens<T, V, false>;
-      kernel<<<ceil_div(tokens, kRouteWarps), kRouteWarps * 32, 0, stream>>>(
-          grad_weights, static_cast<const T*>(logits.ptr), logits.stride, words, weights, chosen, tokens, experts, top_k,
-          static_cast<T*>(grad_logits.ptr), grad_logits.stride);
+      launch_after(kernel, ceil_div(tokens, kRouteWarps), kRouteWarps * 32, stream, grad_weights,
+                   static_cast<const T*>(logits.ptr), logits.stride, words, weights, chosen, tokens, experts, top_k,
+                   static_cast<T*>(grad_logits.ptr), grad_logits.stride);
     });
   });
-  PSB_LAUNCH_CHECK();
 }
 
 long long dispatch_rows(long long slots, int experts, int align) {
@@ -651,9 +655,9 @@ void dispatch_launch(int dtype, RowsIn x, Indices chosen, int tokens, int top_k,
     auto* dst = static_cast<unsigned char*>(out.ptr);
     const int words = int(row_bytes / B), lanes_log2 = row_lanes(words, kRowUnroll, 1, 0, tokens);
     if (few)
-      dispatch_few<B><<<grid_x(std::max(1LL, (long long)blanks.blocks() + tokens)), kRowThreads, 0, stream>>>(
-          src, x.stride * size, chosen.ptr, chosen.wide, int(n), align, position, offsets, counts, blanks, top_k, words, dst,
-          out.stride * size);
+      launch_after(dispatch_few<B>, grid_x(std::max(1LL, (long long)blanks.blocks() + tokens)), kRowThreads, stream, src,
+                   x.stride * size, chosen.ptr, chosen.wide, int(n), align, position, offsets, counts, blanks, top_k, words, dst,
+                   out.stride * size);
     else
       launch_after(dispatch_rows_kernel<B>, grid_x(blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2)), kRowThreads, stream, src, x.stride * size, position, blanks, tokens,
                    top_k, words, dst, out.stride * size, lanes_log2);
@@ -664,7 +668,6 @@ void dispatch_launch(int dtype, RowsIn x, Indices chosen, int tokens, int top_k,
   if (fits(16)) run(Count<16>());
   else if (fits(4)) run(Count<4>());
   else run(Count<2>());
-  PSB_LAUNCH_CHECK();
 }
 
 void combine_launch(int dtype, RowsIn y, long long rows, const int* position, const float* weights, RowsIn add, int tokens,
@@ -682,15 +685,13 @@ void combine_launch(int dtype, RowsIn y, long long rows, const int* position, co
       const int lanes_log2 = row_lanes(width, N, 2, decltype(shape)::kLeastLanesLog2, tokens);
       const unsigned blocks = grid_x(ceil_div_ll(tokens, kRowThreads >> lanes_log2));
       auto run = [&](auto kernel) {
-        kernel<<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(y.ptr), y.stride, rows, position, weights,
-                                                   static_cast<const T*>(add.ptr), add.stride, tokens, top_k, width,
-                                                   static_cast<T*>(out.ptr), out.stride, lanes_log2);
+        launch_after(kernel, blocks, kRowThreads, stream, static_cast<const T*>(y.ptr), y.stride, rows, position, weights,
+                     static_cast<const T*>(add.ptr), add.stride, tokens, top_k, width, static_cast<T*>(out.ptr), out.stride, lanes_log2);
       };
       if (top_k > 2) run(weights ? combine_rows<T, N, W, S, true, 4, 1> : combine_rows<T, N, W, S, false, 4, 1>);
       else run(weights ? combine_rows<T, N, W, S, true, 2, 2> : combine_rows<T, N, W, S, false, 2, 2>);
     });
   });
-  PSB_LAUNCH_CHECK();
 }
 
 void combine_grad_launch(int dtype, RowsIn grad, RowsIn y, long long rows, const int* position, const int* offsets,
@@ -709,9 +710,9 @@ void combine_grad_launch(int dtype, RowsIn grad, RowsIn y, long long rows, const
       const int lanes_log2 = row_lanes(width, N, 8, 5, tokens);
       const unsigned blocks = grid_x(blanks.blocks() + ceil_div_ll(tokens, kRowThreads >> lanes_log2));
       auto run = [&](auto kernel) {
-        kernel<<<blocks, kRowThreads, 0, stream>>>(static_cast<const T*>(grad.ptr), grad.stride, static_cast<const T*>(y.ptr), y.stride,
-                                                   position, blanks, weights, tokens, top_k, width, static_cast<T*>(grad_y.ptr),
-                                                   grad_y.stride, grad_weights, lanes_log2);
+        launch_after(kernel, blocks, kRowThreads, stream, static_cast<const T*>(grad.ptr), grad.stride, static_cast<const T*>(y.ptr),
+                     y.stride, position, blanks, weights, tokens, top_k, width, static_cast<T*>(grad_y.ptr), grad_y.stride, grad_weights,
+                     lanes_log2);
       };
       if constexpr (W == N) {
         if (top_k > 4) run(combine_grad_rows<T, N, W, S, 8, 1>);
@@ -723,7 +724,6 @@ void combine_grad_launch(int dtype, RowsIn grad, RowsIn y, long long rows, const
       }
     });
   });
-  PSB_LAUNCH_CHECK();
 }
 
 }  // namespace psb

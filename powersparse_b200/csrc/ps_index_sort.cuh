@@ -22,6 +22,7 @@
 #include <utility>
 
 #include "ps_common.cuh"
+#include "ps_rows.cuh"
 
 namespace psb {
 
@@ -256,29 +257,7 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
 // with 4, 19.3 with 8).
 inline int sort_blocks(long long n) { return n <= 2048 ? 1 : n <= 4096 ? 4 : n <= 8192 ? 8 : kSortBlocks; }
 
-// A kernel launched with launch_after may start while the one before it still runs; it
-// waits here before it touches what that one writes, and reads that with plain loads
-// (the read-only path may hold lines from before the wait).  let_next_start() in the earlier
-// kernel lets the later one's blocks take their places as soon as every block of the
-// earlier one has its own.
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-template <typename... Params, typename... Args>
-void launch_after(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Args&&... args) {
-  cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
-  config.blockDim = dim3(threads);
-  config.stream = stream;
-  cudaLaunchAttribute attr[1] = {};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attr;
-  config.numAttrs = 1;
-  PSB_CUDA(cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...));
-}
-
-// Launches `kernel` with `clusters` clusters of `blocks` blocks of kSortThreads.
+// As launch_after, with `clusters` clusters of `blocks` blocks of kSortThreads.
 constexpr int kSortSmem = 220 << 10;  // what the most digits and the longest kept strips of 8-byte elements take, and some
 template <auto kernel, typename... Args>
 void launch_clusters(int blocks, long long clusters, size_t smem, cudaStream_t stream, Args... args) {
@@ -297,12 +276,14 @@ void launch_clusters(int blocks, long long clusters, size_t smem, cudaStream_t s
   config.blockDim = dim3(kSortThreads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  cudaLaunchAttribute attr[1] = {};
+  cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = blocks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
-  config.numAttrs = 1;
+  config.numAttrs = 2;
   PSB_CUDA(cudaLaunchKernelEx(&config, kernel, args...));
 }
 

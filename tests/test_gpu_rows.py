@@ -670,6 +670,60 @@ def test_replayed_graphs_streams_and_two_at_once():
             assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
 
 
+def mixed(s, side):
+    """The operators between kernels, copies and fills of torch, on two streams: each reads what the one before has just
+    written and overwrites what the one before that still read."""
+    main = torch.cuda.current_stream()
+    x = psb.embedding(s["table"], s["tokens"], 2.0)
+    kept = []
+    for i in range(6):
+        x.mul_(-0.5)
+        weights, chosen = psb.route(x[:, :48].contiguous(), 4)
+        rows, plan = psb.dispatch(x, chosen, 48, 8)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            y = torch.empty_like(rows)
+            y.copy_(rows)
+            grads = psb.combine_grad(x, y, plan, weights, out=y)
+        out = torch.zeros_like(x)
+        psb.combine(rows, plan, weights, out=out, add=x)
+        main.wait_stream(side)
+        x.copy_(out)
+        x.add_(psb.dispatch_grad(grads[0], plan))
+        rows.zero_()
+        grad = psb.embedding_grad(x, s["tokens"], 300, 0.5, dtype=F32)
+        kept += [out, grads[1].clone(), grad.clone()]
+        y.fill_(3.0)
+    return kept + [x]
+
+
+def test_between_other_kernels_copies_and_streams():
+    """Eager, with a wait after every call, and captured: the same bits."""
+    for n in (600, 3000):
+        s, side = inputs(31, n), torch.cuda.Stream()
+        with pytest.MonkeyPatch.context() as patch:
+            for name in ("embedding", "route", "dispatch", "combine", "combine_grad", "dispatch_grad", "embedding_grad"):
+                def waited(*args, call=getattr(psb, name), **kwargs):
+                    torch.cuda.synchronize()
+                    result = call(*args, **kwargs)
+                    torch.cuda.synchronize()
+                    return result
+                patch.setattr(psb, name, waited)
+            want = mixed(s, side)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            got = mixed(s, side)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = mixed(s, side)
+        for _ in range(5):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_capture_before_any_eager_call():
     """In a process of its own, each operator's first call is a captured one."""
     code = """
