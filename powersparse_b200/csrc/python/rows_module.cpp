@@ -5,7 +5,7 @@
 // addresses that bind() was given, so that it serves whichever library the package has
 // loaded.  Native because at a serving step's sizes the kernels take a few
 // microseconds, and the same checks in Python with a ctypes call took 14 (24 for
-// dispatch, with its four outputs) against the kernels' 2 to 5; these take 5 (7).
+// dispatch, with its four outputs) against the kernels' 2 to 5; these take 4 (6).
 //
 // Every function takes positional arguments only, checked for their number; rows.py
 // holds the signatures.  ValueError for refused arguments, RuntimeError for CUDA errors.
