@@ -258,14 +258,17 @@ int ps_embedding_grad(const void* grad, int grad_dtype, long long grad_stride, c
  * softmax over all experts (normalize = 0) or over the chosen ones (normalize != 0).
  * logits: [tokens x experts] of `dtype`; weights and chosen: [tokens x top_k], packed.
  * A score of -inf switches an expert off: where fewer than top_k are left, the last
- * choices are -1 with weight 0.  A NaN is never chosen, and it makes the weights of its
- * row NaN, as +inf does.  experts <= 1024, top_k <= min(experts, 32). */
+ * choices are -1 with weight 0.  A NaN is never chosen, and it makes all weights of its
+ * row NaN, as +inf does, those beside a choice of -1 too: a row of NaN alone has no other.
+ * (ps_dispatch drops a choice of -1 and ps_combine skips it, so the row's sum shows no NaN;
+ * the weights and ps_route_grad do.)  experts <= 1024, top_k <= min(experts, 32). */
 int ps_route(const void* logits, int dtype, long long logits_stride, int tokens, int experts, int top_k, int normalize,
              float* weights, int* chosen, void* stream);
 
 /* Gradient of ps_route for the logits, given its outputs and the gradient of the
  * weights.  Writes all of grad_logits (the type of logits).  The logits are read where
- * normalize = 0 only.  grad_weights beside a choice of -1 is not used. */
+ * normalize = 0 only.  grad_weights beside a choice of -1 is not used.  A row whose weights
+ * are NaN has NaN throughout. */
 int ps_route_grad(const float* grad_weights, const void* logits, int dtype, long long logits_stride, const float* weights,
                   const int* chosen, int tokens, int experts, int top_k, int normalize, void* grad_logits,
                   long long grad_logits_stride, void* stream);

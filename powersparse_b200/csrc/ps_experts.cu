@@ -169,7 +169,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* logits
   const float e = lane < found ? expf(g.taken[lane] - top) : 0.f;
   const float total = normalize ? warp_sum(e) : sum;
   if (lane < top_k) {
-    weights[t * top_k + lane] = lane >= found ? 0.f : nan ? NAN : e / total;
+    // A NaN (or +inf, whose total is one) reaches every place, those without a choice too: a
+    // row of nothing else has no choice that could show it.
+    weights[t * top_k + lane] = nan || total != total ? NAN : lane >= found ? 0.f : e / total;
     if (lane >= found) chosen[t * top_k + lane] = -1;
   }
 }
@@ -177,7 +179,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* logits
 // With p the softmax that the weights are shares of, g[e] the gradient of the choice e (0
 // where it was not chosen) and G = sum_j g_j w_j:  d logits[e] = p[e] * (g[e] - G).
 // Shares of all experts: p from the logits, dense.  Shares of the chosen ones
-// (normalize): p is the weights, zero elsewhere, and the logits are not read.  g (or
+// (normalize): p is the weights, zero elsewhere, and the logits are not read; a weight that
+// is NaN makes its whole row NaN, as a NaN of the scores does in the dense form.  g (or
 // w_j (g_j - G)) is spread over the experts in shared memory.  A lane's words stand 32
 // words apart, so that a warp writes whole sectors.  16384 tokens of 256 experts in FP32:
 // 7.8 us, 4.5 TB/s, where handing each choice round the warp took 9.3.
@@ -201,13 +204,15 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const floa
     g = grad[t * top_k + lane];
     w = weights[t * top_k + lane];
   }
+  // The dense form has a NaN of the scores in p; here the weights tell of it.
+  const float unchosen = kNormalize && __any_sync(0xffffffffu, w != w) ? NAN : 0.f;
   if (mine < 0 || mine >= experts) {
     mine = -1 - lane;
     g = w = 0.f;
   }
   float* own = spread[warp];
 #pragma unroll
-  for (int v = 0; v < V; ++v) own[v * 32 + lane] = 0.f;
+  for (int v = 0; v < V; ++v) own[v * 32 + lane] = unchosen;
   __syncwarp();
   const float inner = warp_sum(g * w);
   float value = kNormalize ? w * (g - inner) : g;

@@ -105,7 +105,8 @@ def route(logits, top_k: int, normalize: bool = True, stream=None):
 
     float32 weights and int32 experts, ``[tokens, top_k]``, in descending order of score, of equal scores the lower
     index first.  The weights are softmax shares of the chosen experts, or with ``normalize=False`` of all.  A score
-    of -inf switches an expert off; choices that are left over are -1 with weight 0.
+    of -inf switches an expert off; choices that are left over are -1 with weight 0.  A NaN is never chosen and makes
+    all weights of its row NaN, as +inf does.
     """
     return _native.route(logits, top_k, normalize, _handle(stream, logits))
 

@@ -856,3 +856,27 @@ def test_refusals():
                  lambda: psb.combine_grad(x, y, plan._replace(offsets=plan.counts), w)):
         with pytest.raises(ValueError):
             call()
+
+
+# ------------------------------------------------------------------------------------ contracts of single functions
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("experts", [8, 40, 257])
+def test_a_nan_reaches_every_weight_and_gradient_of_its_row(dtype, normalize, experts):
+    logits = randn(gen(1), 9, experts, dtype=dtype)
+    logits[0] = math.nan                                      # nothing else: no choice is left
+    logits[1], logits[1, 3] = -math.inf, math.nan             # nor here
+    logits[2, 5] = math.nan
+    logits[3, 2:], logits[3, 6] = -math.inf, math.nan         # fewer choices than top_k
+    logits[4, 1:], logits[4, 0] = -math.inf, math.inf
+    logits[5, [1, 4]] = math.inf
+    logits[6] = -math.inf                                     # no expert at all, and no NaN
+    logits[7, 2:] = -math.inf
+    weights, chosen = psb.route(logits, 4, normalize)
+    assert chosen[:2].eq(-1).all() and chosen[6].eq(-1).all() and chosen[3, 2:].eq(-1).all() and chosen[4, 1:].eq(-1).all()
+    assert weights[:6].isnan().all()
+    assert not weights[6].any() and not weights[7, 2:].any() and weights[7:].isfinite().all()
+    for grad in (torch.ones_like(weights), torch.where(chosen < 0, math.nan, 1.0)):  # beside a choice of -1 it is not used
+        got = psb.route_grad(grad, logits, weights, chosen, normalize)
+        assert got[:6].isnan().all() and not got[6].any() and got[7:].isfinite().all()
