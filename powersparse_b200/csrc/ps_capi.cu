@@ -101,6 +101,8 @@ psb::Indices indices_of(const void* ptr, int index_type, long long count, const 
   return {ptr, index_type == PS_I64, count};
 }
 
+constexpr int kMaxAlign = 65536;  // of an expert's first row
+
 void require_experts(int tokens, int experts, int top_k, const char* what) {
   require(tokens >= 0, what, "the number of tokens must be >= 0");
   require(experts >= 1 && experts <= psb::kMaxExperts, what, "the number of experts must be in [1, 1024]");
@@ -369,7 +371,7 @@ int ps_route_grad(const float* grad_weights, const void* logits, int dtype, long
 }
 
 long long ps_dispatch_rows(long long slots, int experts, int align) {
-  if (slots < 0 || slots > 0x7fffffffLL || experts < 1 || align < 1) return -1;
+  if (slots < 0 || slots > 0x7fffffffLL || experts < 1 || experts > psb::kMaxExperts || align < 1 || align > kMaxAlign) return -1;
   return psb::dispatch_rows(slots, experts, align);
 }
 
@@ -380,7 +382,7 @@ int ps_dispatch(const void* x, int dtype, long long x_stride, const void* chosen
     const char* what = "ps_dispatch";
     const int size = size_of(dtype, what);
     require_experts(tokens, experts, top_k, what);
-    require(align >= 1 && align <= 65536, what, "align must be in [1, 65536]");
+    require(align >= 1 && align <= kMaxAlign, what, "align must be in [1, 65536]");
     const long long slots = (long long)tokens * top_k, need = psb::dispatch_rows(slots, experts, align);
     const psb::Indices index = indices_of(chosen, index_type, slots, what);
     require(need <= 0x7fffffffLL, what, "the rows in expert order must be below 2^31");

@@ -115,3 +115,12 @@ def test_ops_are_registered_and_traced_on_meta_tensors():
     assert ops.combine(rows, position, offsets, counts, weights, x).shape == (7, 16)
     grad_y, grad_w = ops.combine_grad(x, rows, position, offsets, counts, weights)
     assert grad_y.shape == rows.shape and grad_w.shape == weights.shape
+
+
+@pytest.mark.parametrize("args", [(-1, 1, 1), (2**31, 1, 1), (1, 0, 1), (1, -1, 1), (1, 1, 0), (1, 1025, 1), (1, 1, 65537), (1, 1, -1)])
+def test_c_dispatch_rows_refuses_what_dispatch_refuses(args):
+    assert psb.load_library().ps_dispatch_rows(*args) == -1
+
+
+def test_c_dispatch_rows_takes_the_largest_arguments():
+    assert psb.load_library().ps_dispatch_rows(1, 1024, 65536) == 65536
