@@ -615,7 +615,7 @@ void route_launch(int dtype, RowsIn logits, int tokens, int experts, int top_k, 
   with_type(dtype, [&](auto t) {
     using T = decltype(t);
     with_scores<T>(experts, fits, [&](auto v, bool words) {
-      launch_after(route_tokens<T, decltype(v)::value>, ceil_div(tokens, kRouteWarps), kRouteWarps * 32, stream,
+      launch_after(route_tokens<T, decltype(v)::value>, grid_x(ceil_div_ll(tokens, kRouteWarps)), kRouteWarps * 32, stream,
                    static_cast<const T*>(logits.ptr), logits.stride, words, tokens, experts, top_k, normalize, weights, chosen);
     });
   });
@@ -633,7 +633,7 @@ void route_grad_launch(int dtype, const float* grad_weights, RowsIn logits, cons
     with_scores<T>(experts, fits, [&](auto v, bool words) {
       constexpr int V = decltype(v)::value;
       auto kernel = normalize ? route_grad_tokens<T, V, true> : route_grad_tokens<T, V, false>;
-      launch_after(kernel, ceil_div(tokens, kRouteWarps), kRouteWarps * 32, stream, grad_weights,
+      launch_after(kernel, grid_x(ceil_div_ll(tokens, kRouteWarps)), kRouteWarps * 32, stream, grad_weights,
                    static_cast<const T*>(logits.ptr), logits.stride, words, weights, chosen, tokens, experts, top_k,
                    static_cast<T*>(grad_logits.ptr), grad_logits.stride);
     });

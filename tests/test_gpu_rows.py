@@ -880,3 +880,19 @@ def test_a_nan_reaches_every_weight_and_gradient_of_its_row(dtype, normalize, ex
     for grad in (torch.ones_like(weights), torch.where(chosen < 0, math.nan, 1.0)):  # beside a choice of -1 it is not used
         got = psb.route_grad(grad, logits, weights, chosen, normalize)
         assert got[:6].isnan().all() and not got[6].any() and got[7:].isfinite().all()
+
+
+def test_route_of_the_most_tokens():
+    """2^31 - 1 tokens, where a block count in 32 bits would overflow; one expert, so every weight is one."""
+    n = 2**31 - 1
+    logits = torch.zeros(n, 1, device="cuda", dtype=BF16)
+    logits[n - 1] = math.nan
+    weights, chosen = psb.route(logits, 1)
+    for part in (slice(0, 2**30), slice(2**30, n - 1)):
+        assert (weights[part] == 1).all() and not chosen[part].any()
+    assert weights[n - 1].isnan() and chosen[n - 1] == -1
+    # normalize=False: p = 1 and the sum of g w is g, so the gradient is zero but for the last row
+    grad = psb.route_grad(weights, logits, weights, chosen, False)
+    for part in (slice(0, 2**30), slice(2**30, n - 1)):
+        assert not grad[part].any()
+    assert grad[n - 1].isnan()
