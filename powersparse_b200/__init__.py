@@ -36,6 +36,7 @@ computing anything on the host.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from typing import Optional, Sequence
 
@@ -44,8 +45,6 @@ import numpy as np
 __all__ = [
     "PowerSparseMatrixGPU", "SpMM", "SDDMM", "SDDMM_csr", "SpMM_values", "edge_softmax_csr", "partition_rows",
     "load_library", "LIB_PATH",
-    "embedding", "embedding_grad", "route", "route_grad", "DispatchPlan", "dispatch_rows", "dispatch",
-    "dispatch_grad", "combine", "combine_grad",
     "GROUP_SIZE", "PS_OK", "PS_ERR_INVALID_ARGUMENT", "PS_ERR_CUDA",
 ]
 
@@ -113,6 +112,8 @@ _SIGNATURES = [
 # Names of powersparse_b200.rows, looked up at their first use: that module needs torch.
 _ROW_OPERATORS = ("embedding", "embedding_grad", "route", "route_grad", "DispatchPlan", "dispatch_rows", "dispatch",
                   "dispatch_grad", "combine", "combine_grad")
+if importlib.util.find_spec("torch"):  # without torch, `from powersparse_b200 import *` gives the rest
+    __all__ += _ROW_OPERATORS
 
 
 def __getattr__(name: str):

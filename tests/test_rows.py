@@ -1,5 +1,9 @@
 """CPU tests of the operators on rows chosen by an index: what the entry points refuse,
 their host arithmetic, and the shapes that tracing sees."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -124,3 +128,18 @@ def test_c_dispatch_rows_refuses_what_dispatch_refuses(args):
 
 def test_c_dispatch_rows_takes_the_largest_arguments():
     assert psb.load_library().ps_dispatch_rows(1, 1024, 65536) == 65536
+
+
+def _without_torch(code):
+    """Runs `code` in a process in which `import torch` fails as where torch is not installed."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", "import sys\nsys.modules['torch'] = None\n" + code], capture_output=True, text=True,
+                         timeout=600, cwd=root)
+    assert run.returncode == 0, run.stdout + run.stderr
+    return run.stdout
+
+
+def test_star_import_without_torch():
+    _without_torch("from powersparse_b200 import *\n"
+                   "assert callable(SpMM) and PS_OK == 0\n"
+                   "assert 'embedding' not in globals()")
