@@ -15,6 +15,7 @@ Outputs (git-ignored, shipped with the tree):
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
@@ -101,7 +102,10 @@ def build_cxx(force: bool = False) -> None:
 
 
 def build_rows_module(force: bool = False) -> str:
-    """The Python module behind powersparse_b200.rows, against the installed torch."""
+    """The Python module behind powersparse_b200.rows, against the installed torch (left out where there is none)."""
+    if not importlib.util.find_spec("torch"):
+        print(f"{os.path.basename(ROWS_MODULE)} is left out: powersparse_b200.rows needs torch, which is not installed", file=sys.stderr)
+        return ROWS_MODULE
     src = os.path.join(CSRC, "python", "rows_module.cpp")
     os.makedirs(LIB, exist_ok=True)
     if force or _stale(ROWS_MODULE, [src, os.path.join(INCLUDE, "powersparse_b200.h")]):

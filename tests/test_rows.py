@@ -143,3 +143,11 @@ def test_star_import_without_torch():
     _without_torch("from powersparse_b200 import *\n"
                    "assert callable(SpMM) and PS_OK == 0\n"
                    "assert 'embedding' not in globals()")
+
+
+def test_build_without_torch(tmp_path):
+    """The libraries and the command line tools build; the module on torch tensors is left out."""
+    _without_torch("from powersparse_b200 import build\n"
+                   f"build.ROWS_MODULE = {str(tmp_path / '_rows.so')!r}\n"
+                   "build.build_all()")
+    assert not list(tmp_path.iterdir())
