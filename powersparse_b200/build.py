@@ -6,7 +6,8 @@
 Outputs (git-ignored, shipped with the tree):
   powersparse_b200/lib/libpowersparse_b200.so  C ABI + CUDA kernels (include/powersparse_b200.h)
   powersparse_b200/lib/libpowersparse_b200_checked.so   the same with bounds-checked kernels
-  powersparse_b200/lib/_rows.so                native part of powersparse_b200.rows (torch tensors)
+  powersparse_b200/lib/_rows.so                native part of powersparse_b200.rows (torch tensors), and in
+                                               _rows.so.built_for the torch and Python it is for
   powersparse_b200/lib/libpowersparse.so       the reference's C++ operator API over the C ABI
   powersparse_b200/bin/powersparse_spmm        drop-in benchmark CLI (SpMM)
   powersparse_b200/bin/powersparse_sddmm       drop-in benchmark CLI (SDDMM)
@@ -108,8 +109,14 @@ def build_rows_module(force: bool = False) -> str:
         return ROWS_MODULE
     src = os.path.join(CSRC, "python", "rows_module.cpp")
     os.makedirs(LIB, exist_ok=True)
-    if force or _stale(ROWS_MODULE, [src, os.path.join(INCLUDE, "powersparse_b200.h")]):
-        import torch
+    import torch
+    from .rows import _THIS_TORCH
+    record = ROWS_MODULE + ".built_for"  # read by rows.py before it loads the module
+    built_for = None
+    if os.path.exists(record):
+        with open(record) as f:
+            built_for = f.read()
+    if force or built_for != _THIS_TORCH or _stale(ROWS_MODULE, [src, os.path.join(INCLUDE, "powersparse_b200.h")]):
         from torch.utils import cpp_extension
         includes = cpp_extension.include_paths() + [sysconfig.get_path("include"), INCLUDE,
                                                     os.path.join(os.path.dirname(CUDA_LIBDIR), "include")]
@@ -117,6 +124,8 @@ def build_rows_module(force: bool = False) -> str:
         _run([HOSTCXX, "-std=c++17", "-O2", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
               *("-I" + i for i in includes), "-o", ROWS_MODULE, src, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
               "-lc10_cuda", "-lc10"])
+        with open(record, "w") as f:
+            f.write(_THIS_TORCH)
     return ROWS_MODULE
 
 

@@ -29,6 +29,7 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sysconfig
 from typing import NamedTuple, Optional
 
 import torch
@@ -39,6 +40,9 @@ __all__ = ["embedding", "embedding_grad", "route", "route_grad", "DispatchPlan",
            "combine", "combine_grad"]
 
 _MODULE_PATH = os.path.join(PKG, "lib", "_rows.so")
+# Beside the module: what it was built for, since its layout of torch's and Python's objects is theirs.
+_BUILT_FOR_PATH = _MODULE_PATH + ".built_for"
+_THIS_TORCH = f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}"
 # The entry points that the native module calls, in the order in which its bind() takes them.
 _ENTRY_POINTS = ("ps_last_error", "ps_embedding", "ps_embedding_grad_workspace", "ps_embedding_grad", "ps_route", "ps_route_grad",
                  "ps_dispatch_rows", "ps_dispatch", "ps_combine", "ps_combine_grad")
@@ -49,6 +53,12 @@ def _load_native():
     """The native module (csrc/python/rows_module.cpp), bound to the library that the package has loaded."""
     if not os.path.exists(_MODULE_PATH):
         raise RuntimeError(f"{_MODULE_PATH} is missing: build it with `python -m powersparse_b200.build`")
+    if os.path.exists(_BUILT_FOR_PATH):
+        with open(_BUILT_FOR_PATH) as f:
+            built_for = f.read()
+        if built_for != _THIS_TORCH:
+            raise RuntimeError(f"{_MODULE_PATH} was built for {built_for}, this is {_THIS_TORCH}: "
+                               "build it again with `python -m powersparse_b200.build`")
     name = "powersparse_b200._rows"
     loader = importlib.machinery.ExtensionFileLoader(name, _MODULE_PATH)
     module = importlib.util.module_from_spec(importlib.util.spec_from_file_location(name, _MODULE_PATH, loader=loader))

@@ -151,3 +151,30 @@ def test_build_without_torch(tmp_path):
                    f"build.ROWS_MODULE = {str(tmp_path / '_rows.so')!r}\n"
                    "build.build_all()")
     assert not list(tmp_path.iterdir())
+
+
+def test_a_module_of_another_torch_is_built_again_and_not_loaded(tmp_path, monkeypatch):
+    from powersparse_b200 import build, rows
+    module = tmp_path / "_rows.so"
+    built = []
+
+    def fake(cmd):
+        built.append(cmd)
+        module.write_bytes(b"")
+    monkeypatch.setattr(build, "ROWS_MODULE", str(module))
+    monkeypatch.setattr(build, "_run", fake)
+    build.build_rows_module()
+    build.build_rows_module()
+    assert len(built) == 1  # fresh
+    record = tmp_path / "_rows.so.built_for"
+    assert torch.__version__ in record.read_text()
+    record.write_text("torch 1.0, cpython-38")
+    monkeypatch.setattr(rows, "_MODULE_PATH", str(module))
+    monkeypatch.setattr(rows, "_BUILT_FOR_PATH", str(record))
+    with pytest.raises(RuntimeError, match="torch 1.0"):
+        rows._load_native()
+    build.build_rows_module()
+    assert len(built) == 2 and torch.__version__ in record.read_text()
+    record.unlink()  # of unknown origin
+    build.build_rows_module()
+    assert len(built) == 3
