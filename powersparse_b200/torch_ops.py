@@ -103,13 +103,21 @@ def sddmm_(handle: int, lhs: torch.Tensor, rhs: torch.Tensor, outs: List[torch.T
 # contiguous first (free where it is already).
 
 
+def _require_padding(table_rows: int, padding: Optional[int]) -> None:
+    """Only the gradient looks at the padding; a bad one is refused before the forward pass."""
+    if padding is not None and not 0 <= padding < table_rows:
+        raise ValueError(f"padding must be a row of the table, in [0, {table_rows})")
+
+
 @torch.library.custom_op("powersparse::embedding", mutates_args=())
 def embedding(table: torch.Tensor, tokens: torch.Tensor, scale: float = 1.0, padding: Optional[int] = None) -> torch.Tensor:
+    _require_padding(table.shape[0], padding)
     return rows.embedding(table, tokens, scale)
 
 
 @embedding.register_fake
 def _(table, tokens, scale=1.0, padding=None):
+    _require_padding(table.shape[0], padding)
     return table.new_empty((*tokens.shape, table.shape[1]))
 
 

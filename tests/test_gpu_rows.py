@@ -896,3 +896,10 @@ def test_route_of_the_most_tokens():
     for part in (slice(0, 2**30), slice(2**30, n - 1)):
         assert not grad[part].any()
     assert grad[n - 1].isnan()
+
+
+def test_embedding_op_refuses_a_padding_outside_the_table_in_the_forward_pass():
+    table, tokens = randn(gen(0), 6, 8).requires_grad_(), torch.arange(6, device="cuda")
+    for padding in (-1, 6):
+        with pytest.raises(ValueError, match="padding"):
+            torch.ops.powersparse.embedding(table, tokens, 1.0, padding)

@@ -178,3 +178,12 @@ def test_a_module_of_another_torch_is_built_again_and_not_loaded(tmp_path, monke
     record.unlink()  # of unknown origin
     build.build_rows_module()
     assert len(built) == 3
+
+
+def test_embedding_op_refuses_a_padding_outside_the_table_in_the_forward_pass():
+    table, tokens = torch.empty(100, 16, device="meta"), torch.empty(5, device="meta", dtype=torch.int64)
+    for padding in (-1, 100, 2**40):
+        with pytest.raises(ValueError, match="padding"):
+            torch.ops.powersparse.embedding(table, tokens, 1.0, padding)
+    for padding in (None, 0, 99):
+        assert torch.ops.powersparse.embedding(table, tokens, 1.0, padding).shape == (5, 16)
