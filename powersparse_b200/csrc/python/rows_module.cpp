@@ -87,6 +87,8 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse(std::string(name) + " must be a CUDA tensor");
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda()) refuse(std::string(name) + " must be a CUDA tensor");
+  // A view whose elements stand in memory with the other sign.
+  if (t.is_neg()) refuse(std::string(name) + " is a negated view: resolve it first (Tensor.resolve_neg)");
   return t;
 }
 

@@ -903,3 +903,20 @@ def test_embedding_op_refuses_a_padding_outside_the_table_in_the_forward_pass():
     for padding in (-1, 6):
         with pytest.raises(ValueError, match="padding"):
             torch.ops.powersparse.embedding(table, tokens, 1.0, padding)
+
+
+def test_negated_views_are_refused_by_the_functions_and_resolved_by_the_ops():
+    """Such a view has the negative bit set and its elements in memory with the other sign."""
+    x, i = randn(gen(0), 6, 8), torch.arange(6, device="cuda")
+    lazy = torch._neg_view(x)
+    assert lazy.is_neg()
+    w, c = psb.route(x, 2)
+    _, plan = psb.dispatch(x, c, 8)
+    y = randn(gen(1), 12, 8)
+    for call in (lambda: psb.embedding(lazy, i), lambda: psb.embedding(x, i, out=torch._neg_view(torch.empty_like(x))),
+                 lambda: psb.embedding_grad(lazy, i, 6), lambda: psb.route(lazy, 2), lambda: psb.route_grad(torch._neg_view(w), x, w, c),
+                 lambda: psb.dispatch(lazy, c, 8), lambda: psb.combine(y, plan, torch._neg_view(w)), lambda: psb.combine(y, plan, add=lazy),
+                 lambda: psb.combine_grad(lazy, y, plan, w), lambda: psb.embedding(x, torch._neg_view(i))):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+    assert torch.equal(torch.ops.powersparse.embedding(lazy, i), -x)
