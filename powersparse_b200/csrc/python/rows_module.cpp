@@ -225,9 +225,11 @@ class WithoutGil {
 
 PyObject* wrap(const at::Tensor& t) { return THPVariable_Wrap(t); }
 
-// An output: the tensor that the caller gave, as the same object, or a new one.
+// An output: the tensor that the caller gave, as the same object and counted as changed
+// (autograd refuses a backward pass that needs what stood there), or a new one.
 PyObject* result(PyObject* given, const Matrix& m) {
   if (given == Py_None) return wrap(m.t);
+  if (!m.t.is_inference()) m.t.unsafeGetTensorImpl()->bump_version();
   Py_INCREF(given);
   return given;
 }

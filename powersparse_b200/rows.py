@@ -17,7 +17,7 @@ that the call allocates belong to that stream, and ordering the inputs before it
 other uses of the outputs after it is the caller's part, as with SpMM.  An ``out`` must
 not overlap the inputs but where its function says so.  Nothing here waits for the
 device, and every call can be captured into a CUDA graph.  These functions take no part
-in autograd.
+in autograd, but a tensor given as ``out`` counts as changed in place there.
 
 The C entry points and their exact contracts are in ``include/powersparse_b200.h``.
 ``powersparse_b200.torch_ops`` registers the same operators, with autograd, as

@@ -920,3 +920,35 @@ def test_negated_views_are_refused_by_the_functions_and_resolved_by_the_ops():
         with pytest.raises(ValueError, match="negated"):
             call()
     assert torch.equal(torch.ops.powersparse.embedding(lazy, i), -x)
+
+
+def test_a_given_out_counts_as_changed():
+    """autograd refuses a backward pass through a tensor that a call has written since, as with torch's own out=."""
+    s = inputs(1)
+    x = psb.embedding(s["table"], s["tokens"])
+    weights, chosen = psb.route(s["logits"], 4)
+    rows, plan = psb.dispatch(x, chosen, 48)
+    table = torch.zeros_like(s["table"])
+    scores = torch.empty_like(s["logits"])
+    grad_w = torch.ones_like(weights)
+    for out, call in ((x, lambda: psb.embedding(s["table"], s["tokens"], out=x)),
+                      (table, lambda: psb.embedding_grad(x, s["tokens"], 300, out=table)),
+                      (table, lambda: psb.embedding_grad(x, s["tokens"], 300, out=table, accumulate=True)),
+                      (scores, lambda: psb.route_grad(grad_w, s["logits"], weights, chosen, out=scores)),
+                      (rows, lambda: psb.dispatch(x, chosen, 48, out=rows)),
+                      (x, lambda: psb.combine(rows, plan, weights, out=x)),
+                      (x, lambda: psb.dispatch_grad(rows, plan, out=x)),
+                      (rows, lambda: psb.combine_grad(x, rows, plan, weights, out=rows))):
+        before = out._version
+        call()
+        assert out._version > before
+    leaf = torch.ones(300, 72, device="cuda", requires_grad=True)
+    held = leaf * 2
+    loss = (held * held).sum()
+    psb.embedding(s["table"].float(), torch.arange(300, device="cuda"), out=held.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        out = torch.empty_like(x)
+        psb.embedding(s["table"], s["tokens"], out=out)
+    assert torch.equal(psb.embedding(s["table"], s["tokens"], out=out), psb.embedding(s["table"], s["tokens"]))
