@@ -225,10 +225,10 @@ int ps_partition_rows(int row_num, const int* row_ptr, int parts, int* cuts);
  * width <= 2^24); byte offsets are 64-bit.  Sums, products and softmax statistics
  * are FP32, rounded once, to nearest even, where they are stored.  An output must not
  * overlap an input but where it is said.  No call allocates device memory, waits for
- * the device or uses atomics whose order matters: equal inputs at equal alignment give
- * equal bits, and every call can be captured into a graph.  Rows that
- * begin at multiples of 16 bytes, with a width that is a multiple of 16 bytes, are
- * moved 16 bytes a thread; others by smaller words. */
+ * the device or uses atomics whose order matters: equal inputs of equal types and
+ * alignment give equal bits on the same model of GPU, and every call can be captured into
+ * a graph.  Rows that begin at multiples of 16 bytes, with a width that is a multiple of
+ * 16 bytes, are moved 16 bytes a thread; others by smaller words. */
 enum { PS_F32 = 0, PS_BF16 = 1, PS_F16 = 2 }; /* element types */
 enum { PS_I32 = 0, PS_I64 = 1 };              /* index types */
 
@@ -239,9 +239,10 @@ int ps_embedding(const void* table, int dtype, long long rows, int width, long l
                  int index_type, long long n, float scale, void* out, long long out_stride, void* stream);
 
 /* Gradient of ps_embedding for the table: grad_table[v, :] = scale * sum of grad[i, :]
- * over the i with tokens[i] = v, summed in FP32 in an order that the batch alone
- * fixes.  Tokens outside [0, rows), and the token `padding` where that is >= 0, take
- * no part.  accumulate = 0 writes every row of grad_table (zeros where no token
+ * over the i with tokens[i] = v, summed in FP32 in a fixed order: the same for equal
+ * tokens, sizes, types, alignment and model of GPU, but not the order of the batch.
+ * Tokens outside [0, rows), and the token `padding` where that is >= 0, take no part.
+ * accumulate = 0 writes every row of grad_table (zeros where no token
  * is); accumulate != 0 adds to the rows that tokens name and leaves the others.
  * grad_table's type is grad's or PS_F32.  rows <= 2^31 - 2.  workspace: at least
  * ps_embedding_grad_workspace(n, rows, width) bytes of device memory at a multiple
@@ -282,8 +283,8 @@ long long ps_dispatch_rows(long long slots, int experts, int align);
  * [0, experts) is dropped (position -1).  Expert e's rows begin at offsets[e], a
  * multiple of align, and hold its counts[e] tokens in the order of the batch; rows up
  * to offsets[e + 1] are zeros; offsets[experts] is the end.  Rows from there on are set
- * to zeros too (zero_tail != 0) or stay as they were.  rows: [row_count x width] with row_count >= ps_dispatch_rows(tokens *
- * top_k, experts, align).  position: tokens * top_k ints, offsets: experts + 1,
+ * to zeros too (zero_tail != 0) or stay as they were.  rows: [row_count x width] with
+ * row_count >= ps_dispatch_rows(tokens * top_k, experts, align).  position: tokens * top_k ints, offsets: experts + 1,
  * counts: experts.  A token may name an expert twice.  experts <= 1024, top_k <= 32,
  * align <= 65536. */
 int ps_dispatch(const void* x, int dtype, long long x_stride, const void* chosen, int index_type, int tokens, int top_k,
@@ -293,16 +294,17 @@ int ps_dispatch(const void* x, int dtype, long long x_stride, const void* chosen
 /* The experts' rows brought back: out[t, :] = add[t, :] + sum over j of weights[t, j] *
  * y[position[t, j], :], summed in the order of j.  weights NULL: ones, which makes it
  * the gradient of ps_dispatch; add NULL: zeros; add may be out itself.  A position
- * outside [0, row_count) is skipped, and neither its weight nor a row is read for it. */
+ * outside [0, row_count) is skipped: no row is read for it, and its weight, whatever it
+ * is, is not used (weights holds tokens * top_k numbers all the same). */
 int ps_combine(const void* y, int dtype, long long y_stride, long long row_count, const int* position, const float* weights,
                const void* add, long long add_stride, int tokens, int top_k, int width, void* out, long long out_stride,
                void* stream);
 
 /* Gradient of ps_combine for y and the weights: grad_y[position[t, j], :] = weights[t, j]
  * * grad[t, :], grad_weights[t, j] = <grad[t, :], y[position[t, j], :]> (0 for a skipped
- * position).  grad_y may be y itself.  position, offsets and counts are ps_dispatch's: the rows between an
- * expert's tokens and the next expert are set to zeros, and zero_tail says the same
- * of the rows from offsets[experts] on as there.  (The gradient for add is grad itself.) */
+ * position).  grad_y may be y itself.  position, offsets and counts are ps_dispatch's: the
+ * rows between an expert's tokens and the next expert are set to zeros, and zero_tail says
+ * the same of the rows from offsets[experts] on as there.  (The gradient for add is grad itself.) */
 int ps_combine_grad(const void* grad, int dtype, long long grad_stride, const void* y, long long y_stride, long long row_count,
                     const int* position, const int* offsets, const int* counts, int experts, const float* weights, int tokens,
                     int top_k, int width, void* grad_y, long long grad_y_stride, int zero_tail, float* grad_weights, void* stream);
