@@ -5,7 +5,7 @@
 
 Outputs (git-ignored, shipped with the tree):
   powersparse_b200/lib/libpowersparse_b200.so  C ABI + CUDA kernels (include/powersparse_b200.h)
-  powersparse_b200/lib/libpowersparse_b200_checked.so   the same with bounds-checked kernels
+  powersparse_b200/lib/libpowersparse_b200_checked.so   the same with bounds-checked SpMM and SDDMM kernels
   powersparse_b200/lib/_rows.so                native part of powersparse_b200.rows (torch tensors), and in
                                                _rows.so.built_for the torch and Python it is for
   powersparse_b200/lib/libpowersparse.so       the reference's C++ operator API over the C ABI
@@ -38,9 +38,12 @@ CUDA_LIBDIR = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(
     "lib64")
 
 CUDA_LIB = os.path.join(LIB, "libpowersparse_b200.so")
-# The same library with every operator kernel checking the indices it follows
-# (-DPSB_BOUNDS_CHECK; see ps_ops.cu).  For debugging: each operator call waits for
-# its kernels.  Load it with PSB_LIBRARY=<path> (powersparse_b200.load_library).
+# The same library with every kernel of SpMM and SDDMM checking the indices it follows
+# (-DPSB_BOUNDS_CHECK; see ps_ops.cu).  For debugging: each such call waits for its
+# kernels.  The operators on rows chosen by an index are the same in both libraries: their
+# kernels take an index of the caller (a token, a choice, a position, a plan's bound) for
+# an empty place, or clamp it, where it is out of range, in every build.
+# Load it with PSB_LIBRARY=<path> (powersparse_b200.load_library).
 CHECKED_LIB = os.path.join(LIB, "libpowersparse_b200_checked.so")
 CXX_LIB = os.path.join(LIB, "libpowersparse.so")
 ROWS_MODULE = os.path.join(LIB, "_rows.so")

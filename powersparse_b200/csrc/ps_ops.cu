@@ -57,7 +57,7 @@ struct WorksetView {
 
 // --- Bounds-checked build ------------------------------------------------------
 // With PSB_BOUNDS_CHECK defined (lib/libpowersparse_b200_checked.so, built by
-// `python -m powersparse_b200.build`), the operator kernels check every index they
+// `python -m powersparse_b200.build`), the kernels of this file check every index they
 // take from the layout, the task lists or a caller's array before following it.  A
 // bad task is skipped and a bad index is not followed (the access is dropped or
 // redirected to element 0); the first failure is recorded in g_bounds_status, and the

@@ -95,3 +95,30 @@ def test_out_of_range_indices_are_reported_not_followed():
         print("ok")
     """)
     assert "ok" in out
+
+
+def test_checked_build_has_the_row_operators():
+    """They follow no index out of range in any build; both libraries give the same bits, for a plan from anywhere too."""
+    code = textwrap.dedent(f"""
+        import sys
+        sys.path[:0] = [{ROOT!r}, {os.path.join(ROOT, "tests")!r}]
+        import torch
+        import powersparse_b200 as psb
+        import test_gpu_rows as t
+        out = t.run_all(t.inputs(1)) + t.run_all(t.inputs(2, 3000))
+        far = torch.tensor([[0, 2**31 - 1], [-5, 7], [-2**31, 3]], dtype=torch.int32, device="cuda")
+        plan = psb.DispatchPlan(far, far.view(-1)[:3].contiguous(), far.view(-1)[1:3].contiguous())
+        y, w = t.randn(t.gen(5), 4, 24), t.randn(t.gen(6), 3, 2)
+        out += [psb.combine(y, plan, w), *psb.combine_grad(y[:3], y, plan, w, out=torch.zeros_like(y))]
+        torch.cuda.synchronize()
+        print(psb.load_library()._name)
+        for x in out:
+            print(x.shape, x.dtype, x.double().nan_to_num(3.5).sum().item().hex(), (x.double() ** 2).nan_to_num(3.5).sum().item().hex())
+    """)
+    lines = []
+    for env in (dict(os.environ), dict(os.environ, PSB_LIBRARY=CHECKED)):
+        r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600, env=env, cwd=ROOT)
+        assert r.returncode == 0, r.stdout + r.stderr
+        lines.append(r.stdout.splitlines())
+    assert lines[1][0].endswith("_checked.so") and lines[0][0] != lines[1][0]
+    assert lines[0][1:] == lines[1][1:] and len(lines[0]) > 20
