@@ -94,12 +94,6 @@ __device__ __forceinline__ uint2 block_sums_before(uint2 v, uint2* scratch) {
   return make_uint2(scratch[warp].x + inc.x - v.x, scratch[warp].y + inc.y - v.y);
 }
 
-// The cluster's barrier; a cluster of one block needs only the block's.
-__device__ __forceinline__ void sort_barrier(int blocks) {
-  if (blocks == 1) __syncthreads();
-  else cooperative_groups::this_cluster().sync();
-}
-
 // Shared memory of a sort: kSortWarps rows of counters, two sets of block totals (one
 // pass writes one while a slower block may still read the other), the digits' bases,
 // the digits' first places among the block's staged elements, and scratch; then the
@@ -117,7 +111,8 @@ struct SortShared {
         stage(local + digits) {}
 };
 inline size_t sort_smem(int digits) {
-  return kSortWarps * sizeof(uint2) + sizeof(uint32_t) * ((kSortWarps + 4) * (size_t(digits) + (digits & 1)));
+  static_assert((kSortWarps + 4) % 4 == 0, "the staged elements begin at a multiple of 16 bytes");
+  return kSortWarps * sizeof(uint2) + sizeof(uint32_t) * (kSortWarps + 4) * size_t(digits);
 }
 // Bytes of the staged elements of n indices in `blocks` blocks (none where the strips are walked twice).
 inline size_t stage_smem(long long n, int blocks, size_t element) {
@@ -182,7 +177,7 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
     }
     sh.total[parity * digits + d] = sum;
   }
-  sort_barrier(blocks);
+  cluster.sync();
 
   uint32_t count = 0, earlier = 0, own = 0;
   if (d < digits) {
@@ -198,7 +193,7 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
   }
   // No block may end while another reads its totals: where no barrier follows at once,
   // its two halves stand apart.
-  if (kLast && blocks > 1) cluster.barrier_arrive();
+  if (kLast) cluster.barrier_arrive();
   const uint2 begin = block_sums_before(make_uint2(d < digits ? widen(count) : 0u, own), sh.scratch);
   const bool staged = kStage && kept;
   if (d < digits) {
@@ -248,14 +243,14 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
       }
     }
   }
-  if (!kLast) sort_barrier(blocks);
-  else if (blocks > 1) cluster.barrier_wait();
+  if (!kLast) cluster.sync();
+  else cluster.barrier_wait();
 }
 
-// Blocks of the cluster for n indices: one while each warp's strip is short, more as
-// the strips grow (16384 tokens in two passes: 23.7 us with 16, 25.0 with 8; 3000: 19.1
-// with 4, 19.3 with 8).
-inline int sort_blocks(long long n) { return n <= 2048 ? 1 : n <= 4096 ? 4 : n <= 8192 ? 8 : kSortBlocks; }
+// Blocks of the cluster for n indices, more as the strips grow (16384 tokens in two
+// passes: 23.7 us with 16, 25.0 with 8; 3000: 19.1 with 4, 19.3 with 8).  (Up to 2048
+// indices the callers have kernels of their own, kFewTokens and kFewSlots.)
+inline int sort_blocks(long long n) { return n <= 4096 ? 4 : n <= 8192 ? 8 : kSortBlocks; }
 
 // As launch_after, with `clusters` clusters of `blocks` blocks of kSortThreads.
 constexpr int kSortSmem = 220 << 10;  // what the most digits and the longest kept strips of 8-byte elements take, and some

@@ -952,3 +952,12 @@ def test_a_given_out_counts_as_changed():
         out = torch.empty_like(x)
         psb.embedding(s["table"], s["tokens"], out=out)
     assert torch.equal(psb.embedding(s["table"], s["tokens"], out=out), psb.embedding(s["table"], s["tokens"]))
+
+
+@pytest.mark.parametrize("tokens,k,experts,align,kind", [
+    (2049, 1, 1, 1, "any"), (1025, 2, 1, 128, "far"), (2049, 1, 1024, 1, "any"), (700, 3, 1024, 16, "far"), (1024, 4, 1024, 128, "any"),
+    (4097, 1, 1024, 3, "one"), (2731, 3, 1024, 1, "none"), (8193, 1, 1023, 2, "far"), (65537, 2, 1024, 1, "any"), (65537, 2, 1, 7, "far"),
+    (4300, 32, 2, 1, "any")])
+def test_order_of_many_slots_at_the_least_and_the_most_experts(tokens, k, experts, align, kind):
+    """More than 2048 slots (a sort in clusters of 4, 8 and 16 blocks, beyond 131072 by strips that are walked twice)."""
+    test_dispatch_and_combine(tokens, k, experts, align, kind, BF16, 16)
