@@ -961,3 +961,158 @@ def test_a_given_out_counts_as_changed():
 def test_order_of_many_slots_at_the_least_and_the_most_experts(tokens, k, experts, align, kind):
     """More than 2048 slots (a sort in clusters of 4, 8 and 16 blocks, beyond 131072 by strips that are walked twice)."""
     test_dispatch_and_combine(tokens, k, experts, align, kind, BF16, 16)
+
+
+class Guarded:
+    """Tensors inside larger buffers whose other elements hold a number that no call may change (in what is written) or a
+    NaN that would reach the result (in what is read)."""
+
+    def __init__(self):
+        self.kept = []
+
+    def read(self, t, extra=0):
+        buf = torch.full((t.shape[0] + 64, t.shape[1] + extra), math.nan, device="cuda", dtype=t.dtype)
+        view = buf[32: 32 + t.shape[0], : t.shape[1]]
+        view.copy_(t)
+        return view
+
+    def write(self, rows, width, dtype, extra=0):
+        buf = torch.full((rows + 64, width + extra), -77.0, device="cuda", dtype=dtype)
+        self.kept.append((buf, rows, width))
+        return buf[32: 32 + rows, :width]
+
+    def untouched(self):
+        return all((b[:32] == -77).all() and (b[32 + r:] == -77).all() and (b[:, w:] == -77).all() for b, r, w in self.kept)
+
+
+@pytest.mark.parametrize("dtype,width,extra", [(F32, 8, 0), (F32, 1111, 3), (BF16, 64, 0), (BF16, 514, 2), (F16, 515, 0), (F16, 33, 5),
+                                               (BF16, 2056, 8)])
+@pytest.mark.parametrize("k", [1, 2, 5, 8])
+def test_a_plan_that_points_outside_with_what_stands_around(dtype, width, extra, k):
+    """As above, with everything inside larger buffers: values as the formulas have them, nothing read or changed outside."""
+    g, guard = gen(width + k), Guarded()
+    tokens, rows = 37, 60
+    at = torch.arange(tokens * k, device="cuda") * 7 % (5 * rows // 4)  # rows of y; from `rows` on they are outside
+    if tokens * k > rows:  # no row of grad_y from two places
+        at = torch.where(torch.arange(tokens * k, device="cuda") < rows, at, rows + at)
+    bad = torch.tensor([rows, -1, 2**31 - 1, -2**31, rows + 1, -rows], device="cuda")
+    pick = torch.rand(tokens * k, generator=g, device="cuda") < 0.3
+    at = torch.where(pick, bad[torch.arange(tokens * k, device="cuda") % len(bad)], at).view(tokens, k)
+    nothing = torch.tensor([2**31 - 1, -9, -2**31], dtype=torch.int32, device="cuda")  # by these bounds no row is to be cleared
+    plan = psb.DispatchPlan(at.to(torch.int32).contiguous(), nothing, torch.tensor([2**31 - 1, -2**31], dtype=torch.int32, device="cuda"))
+    y, add, grad = (randn(g, n, width, dtype=dtype) for n in (rows, tokens, tokens))
+    weights = torch.rand(tokens, k, generator=g, device="cuda")
+    token, choice = ((at >= 0) & (at < rows)).nonzero(as_tuple=True)
+    slot = at[token, choice]
+    assert len(slot) and len(slot.unique()) == len(slot)
+    weights[(at < 0) | (at >= rows)] = math.nan
+    term = y[slot].double() * weights[token, choice].double()[:, None]
+    want = add.double().index_add(0, token, term)
+    size = add.double().abs().index_add(0, token, term.abs())
+    out = guard.write(tokens, width, dtype, extra)
+    psb.combine(guard.read(y, extra), plan, weights, guard.read(add), out=out)
+    check(out, want, size * (k + 2) * U)
+    plain = torch.zeros(tokens, width, dtype=torch.float64, device="cuda")
+    out = guard.write(tokens, width, dtype, extra)
+    psb.dispatch_grad(guard.read(y, extra), plan, out=out)
+    check(out, plain.index_add(0, token, y[slot].double()), plain.index_add(0, token, y[slot].double().abs()) * (k + 2) * U)
+
+    grad_y = guard.write(rows, width, dtype, extra)
+    grad_y.fill_(5.0)
+    want_y = torch.full((rows, width), 5.0, dtype=torch.float64, device="cuda")
+    want_y[slot] = weights[token, choice].double()[:, None] * grad[token].double()
+    got, grad_w = psb.combine_grad(guard.read(grad), guard.read(y, extra), plan, weights, out=grad_y)
+    check(got, want_y, want_y.abs() * U)
+    want_w, size = torch.zeros(tokens, k, dtype=torch.float64, device="cuda"), torch.zeros(tokens, k, dtype=torch.float64, device="cuda")
+    term = grad[token].double() * y[slot].double()
+    want_w[token, choice], size[token, choice] = term.sum(1), term.abs().sum(1)
+    check(grad_w, want_w, size * (width / 32 + 24) * U)
+    # bounds from anywhere, all of them to be cleared
+    for offsets in ([-2**31, 2**31 - 1, -2**31], [0, -5, 2**31 - 1], [2**31 - 1] * 3, [-1] * 3):
+        for counts in ([0, 0], [-2**31, 2**31 - 1], [2**31 - 1, -1]):
+            grad_y = guard.write(rows, width, dtype, extra)
+            psb.combine_grad(guard.read(grad), guard.read(y, extra), psb.DispatchPlan(
+                plan.position, *(torch.tensor(v, dtype=torch.int32, device="cuda") for v in (offsets, counts))), weights, out=grad_y)
+    assert guard.untouched()
+
+
+@pytest.mark.parametrize("dtype,width,extra", [(F32, 20, 0), (F32, 131, 3), (BF16, 64, 8), (BF16, 130, 2), (F16, 33, 0)])
+def test_what_stands_around_the_outputs_stays(dtype, width, extra):
+    guard = Guarded()
+    for n, rows in ((3, 5), (700, 90), (2048, 3000), (2049, 3000), (9000, 257)):
+        g = gen(n)
+        table, tokens = randn(g, rows, width, dtype=dtype), torch.randint(-rows, 2 * rows, (n,), generator=g, device="cuda")
+        out = guard.write(n, width, dtype, extra)
+        psb.embedding(guard.read(table, extra), tokens, out=out)
+        assert torch.equal(out.double(), embedding64(table, tokens, 1.0))
+        want, slack = grad64(out, tokens, rows, 1.0)
+        grad = guard.write(rows, width, F32, extra)
+        psb.embedding_grad(guard.read(out, extra), tokens, rows, out=grad)
+        check(grad, want, slack)
+        psb.embedding_grad(guard.read(out, extra), tokens, rows, out=grad, accumulate=True)
+        chosen = torch.randint(-20, 60, (n, 3), generator=g, device="cuda")
+        position, offsets, _ = order64(chosen, 40, 8)
+        need = psb.dispatch_rows(n * 3, 40, 8)
+        room = guard.write(need, width, dtype, extra)
+        _, plan = psb.dispatch(guard.read(out, extra), chosen, 40, 8, out=room)
+        assert plan.position.view(-1).tolist() == position
+        assert (room[offsets[-1]:] == -77).all() and not (room[:offsets[-1]] == -77).all(1).any()
+        logits = randn(g, n, 40, dtype=dtype)
+        w, c = psb.route(guard.read(logits, extra), 3)
+        scores = guard.write(n, 40, dtype, extra)
+        psb.route_grad(torch.rand(n, 3, generator=g, device="cuda"), guard.read(logits, extra), w, c, out=scores)
+        assert (scores != -77).all()
+    assert guard.untouched()
+
+
+@pytest.mark.parametrize("shards", [4, 16])
+def test_fresh_outputs_where_most_experts_are_elsewhere(shards):
+    """A batch on a GPU that holds few of the experts: all rows behind the last one are zeros in what a call allocates."""
+    g = gen(shards)
+    tokens, k, experts, width = 8192, 8, 64, 136
+    chosen = torch.randint(0, experts, (tokens, k), generator=g, device="cuda") - experts // shards
+    mine = experts // shards
+    x = randn(g, tokens, width, dtype=BF16)
+    for align in (1, 128):
+        junk = torch.full((psb.dispatch_rows(tokens * k, mine, align), width), math.nan, device="cuda", dtype=BF16)
+        del junk  # so that the allocation finds something
+        rows, plan = psb.dispatch(x, chosen, mine, align)
+        end = plan.offsets[-1].item()
+        assert plan.counts.sum().item() == ((chosen >= 0) & (chosen < mine)).sum().item() < tokens * k // 2
+        assert end < len(rows) // 2 and not rows[end:].any()
+        token, choice = (plan.position >= 0).nonzero(as_tuple=True)
+        slot = plan.position[token, choice].long()
+        assert torch.equal(rows[slot], x[token])
+        weights = torch.rand(tokens, k, generator=g, device="cuda")
+        junk = torch.full_like(rows, math.nan)
+        del junk
+        grad_y, grad_w = psb.combine_grad(x, rows, plan, weights)
+        want = torch.zeros(len(rows), width, dtype=torch.float64, device="cuda")
+        want[slot] = weights[token, choice].double()[:, None] * x[token].double()
+        check(grad_y, want, want.abs() * U)
+        assert not grad_w[plan.position < 0].any()
+
+
+@pytest.mark.parametrize("weighted", [True, False])
+def test_combine_gradient_where_not_every_input_takes_one(weighted):
+    """The registered op with weights, rows or something added that take no gradient: the same gradients for the others."""
+    g = gen(13)
+    ops = torch.ops.powersparse
+    chosen = torch.randint(-1, 7, (50, 3), generator=g, device="cuda")
+    x, add = randn(g, 50, 24), randn(g, 50, 24)
+    weights = torch.rand(50, 3, generator=g, device="cuda") if weighted else None
+    _, plan = psb.dispatch(x, chosen, 7, 4)
+    y = randn(g, psb.dispatch_rows(150, 7, 4), 24)
+    probe = randn(g, 50, 24)
+    grad_y, grad_w = psb.combine_grad(probe, y, plan, weights if weighted else torch.ones(50, 3, device="cuda"))
+    wants = dict(y=grad_y, weights=grad_w, add=probe)
+    for names in (("y",), ("weights",), ("add",), ("y", "add"), ("y", "weights"), ("weights", "add"), ("y", "weights", "add")):
+        if not weighted and "weights" in names:
+            continue
+        args = {n: t.clone().requires_grad_(n in names) for n, t in (("y", y), ("weights", weights), ("add", add)) if t is not None}
+        out = ops.combine(args["y"], *plan, args.get("weights"), args["add"])
+        assert torch.equal(out, psb.combine(y, plan, weights, add))
+        (out * probe).sum().backward()
+        for n, t in args.items():
+            assert (t.grad is not None) == (n in names)
+            assert n not in names or torch.equal(t.grad, wants[n])
