@@ -246,7 +246,8 @@ int ps_embedding(const void* table, int dtype, long long rows, int width, long l
  * is); accumulate != 0 adds to the rows that tokens name and leaves the others.
  * grad_table's type is grad's or PS_F32.  rows <= 2^31 - 2.  workspace: at least
  * ps_embedding_grad_workspace(n, rows, width) bytes of device memory at a multiple
- * of 256 (-1 for arguments out of range; 0 for small batches, where it may be NULL),
+ * of 256 (-1 for arguments out of range; 0 for small batches of rows that are not too
+ * wide, where it may be NULL),
  * in use until the call has run (by a graph that captured the call, while the graph
  * may run); it needs no initialisation and nothing in it outlives the call. */
 long long ps_embedding_grad_workspace(long long n, long long rows, int width);

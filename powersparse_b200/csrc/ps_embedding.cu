@@ -381,11 +381,20 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_runs(const Item* items, 
 // others end), where less than a block shares a row every groups-th of them a group of
 // threads and then the groups.  Up to kFewTokens / kFewThreads tokens a
 // thread are compared, so no sort is needed, and neither are partial rows.  Behind them
-// the blocks that clear the rows which no token names.  Against the sort and its
-// launches: 1024 tokens, rows of 256, 10.3 us against 18.5; 2048 tokens 14.1 against
-// 20.9 (rows of 2048: 24.5 against 22.7); 4096 tokens 34 against 21, as every block
-// reads every token.
+// the blocks that clear the rows which no token names.
+//
+// Taken up to kFewTokens tokens, as every block reads every token, and up to kFewElements
+// elements, as the few blocks of one token read all of its rows while the sort's sums
+// spread them over the GPU.  Against the sort and its launches, in 16 bits into 4096 rows,
+// tokens as text has them (all of one kind; all distinct): 2048 tokens, rows of 256, 11 us
+// against 20 (32, 22; 14, 17); 4096 tokens 34 against 21; 2048 tokens, rows of 2048, 30
+// against 22 (227, 25; 19, 20); rows of 8192, 512 tokens, 21 against 22 (96, 20; 25, 20), 1024
+// tokens 35 against 26 (198, 23; 38, 25) and 2048 tokens 88 against 31 (779, 30; 49, 29).
+// Where the table is large its clearing hides the sums of few tokens, and the border lies
+// higher: 134M elements, rows of 8192, 600 tokens 52 against 55, 1100 tokens 62 against 56.
 constexpr int kFewTokens = 2048;
+constexpr long long kFewElements = 5 << 20;
+inline bool few_tokens_suffice(long long n, int width) { return n <= kFewTokens && n * width <= kFewElements; }
 constexpr int kFewThreads = 256;
 constexpr int kFewEach = kFewTokens / kFewThreads;
 constexpr int kFewWarps = kFewThreads / 32;
@@ -550,7 +559,7 @@ void embedding_launch(int dtype, RowsIn table, long long rows, int width, Indice
 }
 
 size_t embedding_grad_workspace(long long tokens, long long rows, int width) {
-  return tokens <= kFewTokens ? 0 : Workspace(tokens, rows, width).bytes;
+  return few_tokens_suffice(tokens, width) ? 0 : Workspace(tokens, rows, width).bytes;
 }
 
 void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float scale, long long padding, bool accumulate,
@@ -564,7 +573,7 @@ void embedding_grad_launch(int grad_dtype, RowsIn grad, Indices tokens, float sc
   const Joins joins{reinterpret_cast<Item*>(ws + at.shorter), reinterpret_cast<Item*>(ws + at.longer),
                     reinterpret_cast<int*>(ws + at.join_count)};
   auto* partial = reinterpret_cast<float*>(ws + at.partial);
-  const bool few = n <= kFewTokens;
+  const bool few = few_tokens_suffice(n, width);
   const long long row_bytes = (long long)width * out_size;
   // A gradient of more than kClearFirst + kClearLast bytes is cleared in three parts, so
   // that the sums and the joins, too, run beside a part of it.

@@ -248,8 +248,8 @@ __device__ __forceinline__ void sort_pass(SortShared sh, int digits, int parity,
 }
 
 // Blocks of the cluster for n indices, more as the strips grow (16384 tokens in two
-// passes: 23.7 us with 16, 25.0 with 8; 3000: 19.1 with 4, 19.3 with 8).  (Up to 2048
-// indices the callers have kernels of their own, kFewTokens and kFewSlots.)
+// passes: 23.7 us with 16, 25.0 with 8; 3000: 19.1 with 4, 19.3 with 8).  (For fewer the
+// callers have kernels of their own, by kFewTokens and kFewSlots; wide rows alone come here.)
 inline int sort_blocks(long long n) { return n <= 4096 ? 4 : n <= 8192 ? 8 : kSortBlocks; }
 
 // As launch_after, with `clusters` clusters of `blocks` blocks of kSortThreads.

@@ -1116,3 +1116,19 @@ def test_combine_gradient_where_not_every_input_takes_one(weighted):
         for n, t in args.items():
             assert (t.grad is not None) == (n in names)
             assert n not in names or torch.equal(t.grad, wants[n])
+
+
+@pytest.mark.parametrize("kind", ["one", "skewed", "distinct", "any", "empty"])
+@pytest.mark.parametrize("n,width,rows", [(1, 5 * 2**20, 2), (1, 5 * 2**20 + 8, 3), (2, 5 * 2**19 + 1, 3), (33, 163841, 40), (200, 26300, 257),
+                                          (1024, 5120, 1500), (1025, 5120, 1500), (2048, 2560, 3000), (2048, 2568, 3000),
+                                          (2047, 2563, 2047)])
+def test_embedding_grad_of_few_tokens_in_wide_rows(kind, n, width, rows):
+    """About the border of 5 * 2^20 elements between the one launch and the sort, which fewer than 2049 tokens reach by wide rows alone."""
+    g = gen(n)
+    tokens, grad = batch(g, kind, n, rows), randn(g, n, width, dtype=BF16)
+    want, slack = grad64(grad, tokens, rows, 0.5)
+    for out in (BF16, F32):
+        check(psb.embedding_grad(grad, tokens, rows, 0.5, dtype=out), want, slack)
+    dst = torch.zeros(rows, width, device="cuda")
+    psb.embedding_grad(grad, tokens, rows, 0.5, out=dst, accumulate=True)
+    check(dst, want, slack)

@@ -187,3 +187,12 @@ def test_embedding_op_refuses_a_padding_outside_the_table_in_the_forward_pass():
             torch.ops.powersparse.embedding(table, tokens, 1.0, padding)
     for padding in (None, 0, 99):
         assert torch.ops.powersparse.embedding(table, tokens, 1.0, padding).shape == (5, 16)
+
+
+def test_embedding_grad_of_few_tokens_in_wide_rows_is_sorted():
+    """The one launch for few tokens (no workspace) adds up a token's rows in few blocks: not for more than 5 * 2^20 elements."""
+    size = psb.load_library().ps_embedding_grad_workspace
+    for n, width in ((2048, 2560), (1024, 5120), (1, 5 * 2**20), (2047, 2560), (0, 2**24)):
+        assert size(n, 4096, width) == 0, (n, width)
+    for n, width in ((2048, 2561), (2048, 8192), (1025, 5120), (1, 5 * 2**20 + 1), (2049, 1)):
+        assert size(n, 4096, width) > 0, (n, width)
