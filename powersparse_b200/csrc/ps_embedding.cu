@@ -18,8 +18,8 @@ namespace {
 
 // ---- lookup ---------------------------------------------------------------------
 // 2^lanes_log2 threads a row, kRowUnroll words of it in flight each.  Bound by memory:
-// 16384 tokens of 4096 in 16 bits take 31 us, 6.1 TB/s of the 189 MB that have to move;
-// 16 tokens 2.1 us, a launch.
+// 16384 tokens of 4096 in 16 bits take 32 us with inputs that alternate, 5.9 TB/s of the
+// 189 MB that have to move (30 with inputs that stay); 16 tokens 2.1 us, a launch.
 constexpr int kRowThreads = 256;
 constexpr int kRowUnroll = 4;
 
@@ -212,9 +212,9 @@ struct Joins {
 
 // Bound by memory where the rows are wide and the table large (16384 tokens of 2048 in
 // 16 bits into 131072 rows in 32: 176 us for sort, sums, joins and clearing together, 98%
-// of the copy rate).  Ragged rows (50003 of 515 in 16 bits, 40 us in all) are bound by
-// latency and instructions: 21 us for the sort's two passes, about 11 for the sums, 8
-// for the joins.  Eight rows in flight and eight blocks an SM: sixteen rows or ten blocks
+// of the copy rate).  Ragged rows (50003 of 515 in 16 bits, 47 us in all with inputs that
+// alternate, 40 with inputs that stay in the L2) are bound by latency and instructions: 21 us
+// for the sort's two passes, about 11 of the 40 for the sums, 8 for the joins.  Eight rows in flight and eight blocks an SM: sixteen rows or ten blocks
 // took 2 and 6 us longer there.
 constexpr int kSumThreads = 128;
 constexpr int kMaxChunk = 64;

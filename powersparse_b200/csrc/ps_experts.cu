@@ -62,9 +62,10 @@ struct Gathered {
 // bound that at least k scores reach, and rarely many more do: those are gathered in
 // shared memory, where each lane ranks one of them among all.  Where more than 32 reach
 // it, the scores are taken one by one instead.
-// 16384 tokens of 256 experts in FP32, top 8: 8.3 us, 2.1 TB/s; bound by instructions
-// (about 400 a warp, 72% of the issue slots taken).  A maximum over the warp for each
-// choice took 17.3 us; half a warp a token the same as a whole one.
+// 16384 tokens of 256 experts in FP32, top 8: 7.8 us a call with the scores in the L2, 8.9
+// with scores from memory (1.9 TB/s); in 16 bits 9.1, as it is bound by instructions (about
+// 400 a warp, 75% of the issue slots taken).  A maximum over the warp for each choice took
+// 17.3 us; half a warp a token the same as a whole one.
 template <int V, typename Take>
 __device__ __forceinline__ int top_scores(float (&x)[V], int top_k, Gathered& g, float& top, Take&& take) {
   const int lane = threadIdx.x & 31;
@@ -182,8 +183,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* logits
 // (normalize): p is the weights, zero elsewhere, and the logits are not read; a weight that
 // is NaN makes its whole row NaN, as a NaN of the scores does in the dense form.  g (or
 // w_j (g_j - G)) is spread over the experts in shared memory.  A lane's words stand 32
-// words apart, so that a warp writes whole sectors.  16384 tokens of 256 experts in FP32:
-// 7.8 us, 4.5 TB/s, where handing each choice round the warp took 9.3.
+// words apart, so that a warp writes whole sectors.  16384 tokens of 256 experts in FP32,
+// dense: 7.4 us with the scores in the L2, 8.6 from memory (4.1 TB/s), where handing each
+// choice round the warp took 9.3; normalized 6.6.
 template <typename T, int V, bool kNormalize>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const float* grad, const T* logits,
                                                                       long long stride, bool words, const float* weights,
@@ -423,9 +425,9 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsign
 // A token's rows are added up in the order of the choices, kSlots of them at a time and
 // kTurns stretches of the row, so that a thread has four loads in flight whether a token
 // has many rows or two.  Bound by memory: 8192 tokens of 4096 in 16 bits, 8 experts each
-// and a residual take 108 us, 6.2 TB/s (the positions and weights of a batch are read
-// before its rows: 111 otherwise; eight rows in flight: 112, and 103 against 81 in 32
-// bits, where they cost occupancy).  6799 tokens with 2 experts each: 32 us with (2, 2),
+// and a residual take 113 us with inputs that alternate, 5.9 TB/s, and 108 with inputs that
+// stay (the positions and weights of a batch are read before its rows: 111 otherwise;
+// eight rows in flight: 112, and 103 against 81 in 32 bits, where they cost occupancy).  6799 tokens with 2 experts each: 32 us with (2, 2),
 // 41 with (4, 1).
 template <typename T, int N, int W, int S, bool kWeighted, int kSlots, int kTurns>
 __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* y, long long y_stride, long long rows,

@@ -10,7 +10,8 @@
     combine_grad(grad, y, plan, weights)           its gradients for the rows and the weights
 
 Matrices are float32, bfloat16 or float16 tensors whose rows are contiguous (any row
-stride of at least the width); indices are int32 or int64.  ``stream`` is a torch
+stride of at least the width); indices are int32 or int64, and they, weights and plans are
+contiguous.  ``stream`` is a torch
 stream or a raw handle; without it a call runs on PyTorch's current stream of the
 tensors' device, which need not be the current device.  With it, outputs and scratch
 that the call allocates belong to that stream, and ordering the inputs before it and

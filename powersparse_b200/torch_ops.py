@@ -17,6 +17,9 @@ and the operators on rows chosen by an index (``powersparse_b200.rows``), differ
     combine(y, position, offsets, counts, weights, add) -> out
 
 with their gradients as ops of their own (embedding_grad, route_grad, combine_grad).
+An op costs its caller about 10 us more than the function of ``rows`` behind it, and 24
+more where a gradient is wanted; outputs are always new tensors, zeros behind the last
+expert's rows included.  A gradient has the type of its input.
 
 Fake (meta) implementations give shapes for tracing; they read the matrix's
 dimensions through the C ABI.  Importing this module registers the ops once.
