@@ -1132,3 +1132,29 @@ def test_embedding_grad_of_few_tokens_in_wide_rows(kind, n, width, rows):
     dst = torch.zeros(rows, width, device="cuda")
     psb.embedding_grad(grad, tokens, rows, 0.5, out=dst, accumulate=True)
     check(dst, want, slack)
+
+
+@pytest.mark.parametrize("handle", [False, True])
+def test_explicit_stream_of_every_function_with_outputs_given(handle):
+    """More than 2048 tokens (a workspace on that stream), a torch stream or its handle, and every ``out``."""
+    s = inputs(17, 3000)
+    want = run_all(s)
+    grad_scores = psb.route_grad(want[10], s["logits"], want[2], want[3])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    on = side.cuda_stream if handle else side
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # what is given belongs to that stream too
+        x, table, scores = torch.empty_like(want[0]), torch.empty_like(want[1]), torch.empty_like(s["logits"])
+        rows, y, grad_y, grad_x = (torch.zeros_like(want[i]) for i in (4, 8, 9, 11))
+    psb.embedding(s["table"], s["tokens"], 2.0, out=x, stream=on)
+    psb.embedding_grad(x, s["tokens"], 300, 0.5, out=table, stream=on)
+    weights, chosen = psb.route(s["logits"], 4, stream=on)
+    _, plan = psb.dispatch(x, chosen, 48, 8, out=rows, stream=on)
+    psb.combine(rows, plan, weights, x, out=y, stream=on)
+    _, grad_w = psb.combine_grad(y, rows, plan, weights, out=grad_y, stream=on)
+    psb.dispatch_grad(grad_y, plan, out=grad_x, stream=on)
+    psb.route_grad(grad_w, s["logits"], weights, chosen, out=scores, stream=on)
+    side.synchronize()
+    for got, ref in zip((x, table, weights, chosen, rows, *plan, y, grad_y, grad_w, grad_x, scores), [*want[:12], grad_scores]):
+        assert torch.equal(got, ref)
