@@ -214,8 +214,8 @@ struct Joins {
 // 16 bits into 131072 rows in 32: 176 us for sort, sums, joins and clearing together, 98%
 // of the copy rate).  Ragged rows (50003 of 515 in 16 bits, 47 us in all with inputs that
 // alternate, 40 with inputs that stay in the L2) are bound by latency and instructions: 21 us
-// for the sort's two passes, about 11 of the 40 for the sums, 8 for the joins.  Eight rows in flight and eight blocks an SM: sixteen rows or ten blocks
-// took 2 and 6 us longer there.
+// for the sort's two passes, about 11 of the 40 for the sums, 8 for the joins.  Eight rows
+// in flight and eight blocks an SM: sixteen rows or ten blocks took 2 and 6 us longer there.
 constexpr int kSumThreads = 128;
 constexpr int kMaxChunk = 64;
 

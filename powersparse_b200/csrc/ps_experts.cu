@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_tokens(const T* logits
   const float e = lane < found ? expf(g.taken[lane] - top) : 0.f;
   const float total = normalize ? warp_sum(e) : sum;
   if (lane < top_k) {
-    // A NaN (or +inf, whose total is one) reaches every place, those without a choice too: a
-    // row of nothing else has no choice that could show it.
+    // A NaN (or +inf, which makes the total NaN) reaches every place, those without a choice
+    // too: a row of NaN alone has no choice that could show it.
     weights[t * top_k + lane] = nan || total != total ? NAN : lane >= found ? 0.f : e / total;
     if (lane >= found) chosen[t * top_k + lane] = -1;
   }
@@ -234,9 +234,9 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_grad_tokens(const floa
 #pragma unroll
     for (int v = 0; v < V; ++v) sum += p[v] = expf(x.get(v) - top);
     sum = warp_sum(sum);
-    // (a NaN stays.)  One rounding to 32 bits more than a division of each p, which took 9.2
-    // to 9.8 us where this takes 7.4 (16384 tokens of 256 experts).
-    sum = sum > 0.f ? 1.f / sum : sum;
+    // One rounding to 32 bits more than a division of each p, which took 9.2 to 9.8 us where
+    // this takes 7.4 (16384 tokens of 256 experts).
+    sum = sum > 0.f ? 1.f / sum : sum;  // a NaN stays
   }
   Pack<T, V, W> o;
 #pragma unroll
@@ -427,8 +427,8 @@ __global__ void __launch_bounds__(kRowThreads) dispatch_rows_kernel(const unsign
 // has many rows or two.  Bound by memory: 8192 tokens of 4096 in 16 bits, 8 experts each
 // and a residual take 113 us with inputs that alternate, 5.9 TB/s, and 108 with inputs that
 // stay (the positions and weights of a batch are read before its rows: 111 otherwise;
-// eight rows in flight: 112, and 103 against 81 in 32 bits, where they cost occupancy).  6799 tokens with 2 experts each: 32 us with (2, 2),
-// 41 with (4, 1).
+// eight rows in flight: 112, and 103 against 81 in 32 bits, where they cost occupancy).
+// 6799 tokens with 2 experts each: 32 us with (2, 2), 41 with (4, 1).
 template <typename T, int N, int W, int S, bool kWeighted, int kSlots, int kTurns>
 __global__ void __launch_bounds__(kRowThreads) combine_rows(const T* y, long long y_stride, long long rows,
                                                             const int* position, const float* weights,
